@@ -256,6 +256,22 @@ int wb_bn_relu_pool_fwd(WbBackend* b, const float* x, int64_t n, int64_t c, int6
 int wb_bn_relu_pool_bwd(WbBackend* b, const float* x, const float* dy_pooled, int64_t n, int64_t c, int64_t h, int64_t w,
                         const float* gamma, const float* beta, const float* save_mean, const float* save_rstd, float* dx,
                         float* dgamma, float* dbeta, float* dbias_conv);
+/* F::layer_norm (crates/weta-nn/src/functional.rs:183-195) over the last `normalized_dims` dims of a strided f32 or
+ * f64 view: y = (x - mean) * rstd * weight + bias with the biased variance and rstd = 1 / sqrt(var + eps).  weight and
+ * bias are contiguous, of the normalised dims' size and x's dtype; either may be NULL, and so may save_mean / save_rstd
+ * (one value per row, for the backward pass).  y is contiguous in x's shape.  No output may overlap another operand
+ * (WB_ERR_INVALID).  Results do not change from run to run. */
+int wb_layer_norm_fwd(WbBackend* b, const WbView* x, int normalized_dims, const void* weight, const void* bias, double eps, void* y,
+                      void* save_mean, void* save_rstd);
+/* The gradient autograd derives through that chain: dx (contiguous in x's shape, the gradient of the view: for a
+ * broadcast view the caller sums it), dweight = sum over the rows of dy * xhat, dbias = sum of dy.  Any of the three
+ * may be NULL.  x and dy share one shape, their strides may differ.  dweight / dbias need a workspace of
+ * wb_layer_norm_bwd_workspace(b, rows, cols, dtype) bytes (-1: bad arguments), aligned to 16 bytes, which the caller owns:
+ * calls that may run at the same time (two streams, two captured graphs) need one each.  With no rows dweight and
+ * dbias are zeroed. */
+int64_t wb_layer_norm_bwd_workspace(const WbBackend* b, int64_t rows, int64_t cols, int dtype);
+int wb_layer_norm_bwd(WbBackend* b, const WbView* x, const WbView* dy, int normalized_dims, const void* weight, const void* save_mean,
+                      const void* save_rstd, void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes);
 /* F::linear (crates/weta-nn/src/functional.rs:54-60): y[n, out] = x[n, in] * weight[out, in]^T + bias (bias may be
  * NULL; relu != 0 applies ReLU in the same pass), in the backend's matmul mode.  Backward (MatmulBw,
  * crates/weta-autograd/src/ops.rs:821-827, and the bias's sum over the batch, ops.rs:46-58): dweight[out, in] =
@@ -360,6 +376,47 @@ int wb_trainer_read_loss(WbTrainer* t, float* host_loss);
  * the report waits for the stream and returns lines "label calls total_ms". */
 int wb_trainer_set_timing(WbTrainer* t, int on);
 const char* wb_trainer_timing_report(WbTrainer* t);
+
+/* ---- Adam over many tensors --------------------------------------------------------------------
+ * The optimizer's walk over its parameter list (crates/weta-optim/src/lib.rs:210-239, 276-283) as one launch, with the
+ * state in 32 or in 8 bits, and the 2-norm of all gradients for clipping, which stays on the device.
+ *
+ * State memory is the caller's: wb_adam_multi_state_bytes(lens, n, state_bits) bytes, aligned to 16.  Tensor i owns the
+ * elements [offset_i, offset_i + len_i), offset_i = the sum of the lengths before it, each rounded up to 256; P is the
+ * end of the last one, rounded up likewise.  32 bits: f32 m[P], v[P].  8 bits: int8 codes of m [P], uint8 codes of
+ * sqrt(v) [P], then f32 scales of m [P / 256] and of sqrt(v) [P / 256]: m = s * sign(c) * (c / 127)^2 and
+ * sqrt(v) = s * (c / 255)^2, s the block's largest magnitude; codes are rounded to the nearest on the square root's
+ * scale, and a second moment that is not zero keeps at least code 1.  The update itself uses the new moments before they
+ * are rounded.  A block with a moment that is not finite reads as NaN from then on.  A copy of these bytes and the step
+ * count is all that resuming takes. */
+typedef struct WbAdamMulti WbAdamMulti;
+typedef struct WbAdamTensor {
+    float* theta;
+    int64_t len;
+    int32_t no_decay; /* not 0: exempt from weight decay (biases, gains) */
+    int32_t reserved;
+} WbAdamTensor;
+int64_t wb_adam_multi_state_bytes(const int64_t* lens, int n, int state_bits); /* -1: bad arguments */
+/* Tensors may lie anywhere (4-byte aligned) but not overlap; a length may be 0.  keep_state: the memory holds a saved
+ * state; else it is zeroed.  The handle belongs to the backend, which has to outlive it; a handle's calls do not
+ * overlap each other (one stream, or ordered by the caller). */
+int wb_adam_multi_create(WbBackend* b, const WbAdamTensor* tensors, int n, int state_bits, void* state, int64_t state_bytes, int keep_state,
+                         WbAdamMulti** out);
+int wb_adam_multi_destroy(WbAdamMulti* h);
+int64_t wb_adam_multi_state_len(const WbAdamMulti* h);        /* P */
+int64_t wb_adam_multi_offset(const WbAdamMulti* h, int index); /* offset_i; -1: no such tensor */
+/* The gradients of the following calls, one pointer per tensor (4-byte aligned, not overlapping a parameter).  NULL: the
+ * tensor has none and is left as it is, its state too.  Only the pointers are kept. */
+int wb_adam_multi_set_grads(WbAdamMulti* h, const float* const* grads, int n);
+/* norm = sqrt(sum of all squares), summed in f64 in a fixed order; clip_scale (may be NULL) =
+ * min(1, max_norm / (norm + 1e-6)).  Both are device scalars. */
+int wb_adam_multi_grad_norm(WbAdamMulti* h, double max_norm, float* norm, float* clip_scale);
+/* Step t >= 1 (at t = 1 the old state is not read); lr and the rest may change from step to step.  The gradient is
+ * multiplied by grad_scale (1: not at all) and, where device_grad_scale is not NULL, by that device scalar, the two
+ * multiplied first.  With 32-bit state the results are wb_adam_step's, bit for bit. */
+int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64_t t, double grad_scale, const float* device_grad_scale);
+/* The moments as f32 [P] each (either may be NULL), in the state's order: what 8-bit state stands for. */
+int wb_adam_multi_read_state(WbAdamMulti* h, float* m, float* v);
 
 /* ---- data-parallel training step ---------------------------------------------------------------
  * No counterpart in the reference: its backends are per-ordinal singletons with no gradient exchange

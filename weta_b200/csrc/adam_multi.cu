@@ -1,0 +1,474 @@
+// Adam / AdamW over many tensors in one launch (crates/weta-optim/src/lib.rs:210-239, 276-283, which walks the parameter
+// list), with its state in 32 or in 8 bits, and the 2-norm of all their gradients.
+//
+// State layout: tensor i owns the elements [offset_i, offset_i + len_i), offset_i a multiple of 256.
+//   32 bits: m[P], v[P] as f32 (P: all offsets' end).
+//   8 bits:  codes of m (signed) [P], codes of sqrt(v) (unsigned) [P], then one f32 scale per 256 elements for each.
+// Both codes are companded by a square root, m = s sign(c) (c / 127)^2 and sqrt(v) = s (c / 255)^2 with s the largest
+// magnitude of the block: the distance between neighbouring values is 2 / c of the value, so the large ones, which
+// carry the update, are kept to 0.8 % (m) and 0.4 % (sqrt(v)) and the least one is 6e-5 (1.5e-5) of the largest.
+// sqrt(v) rather than v is coded because it has m's range (v's is twice as many decades) and is at hand in the update.
+// A second moment that is not zero keeps at least code 1: rounding it to zero would leave m / (0 + eps).
+// Compiled with -fmad=false and without approximate functions: every f32 rounding is the one written here, so the
+// codes do not depend on the launch's shape, and the 32-bit step gives wb_adam_step's bits.
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "adam.cuh"
+#include "common.h"
+
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int BLOCK8 = 256;        // elements that share a scale: one warp, eight per lane
+constexpr int64_t CHUNK = 2048;    // elements a thread block takes at a time, all of one tensor
+constexpr float M_TOP = 127.f, V_TOP = 255.f;
+constexpr float TINY = 7.8886090522101181e-31f;  // 2^-100, the least scale: its reciprocal is still finite
+
+struct Tensor {
+    float* theta;
+    const float* grad;
+    int64_t offset;
+    int64_t len;  // negative: -len elements, exempt from weight decay
+};
+
+// The tensors of one launch, passed by value: nothing to upload, nothing a captured graph could lose.
+template <int N>
+struct Table {
+    int n;
+    unsigned int chunks;          // of all tensors together
+    unsigned int first[N];        // a tensor's first chunk
+    Tensor t[N];
+};
+
+// The tensor that holds chunk c: the last one whose first chunk is not behind it (tensors of no chunk share their
+// successor's first one).
+template <int N>
+__device__ __forceinline__ int find_tensor(const Table<N>& tab, unsigned int c) {
+    int lo = 0, hi = tab.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tab.first[mid] <= c) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ AdamK with_device_scale(AdamK k, const float* scale) {
+    if (scale) {
+        const float s = *scale;
+        k.gscale = k.scale_grad ? k.gscale * s : s;
+        k.scale_grad = 1;
+    }
+    return k;
+}
+
+// ---- 32-bit state -------------------------------------------------------------------------------------------
+
+template <int N>
+__global__ void __launch_bounds__(THREADS) adam_multi32_kernel(const __grid_constant__ Table<N> tab, float* __restrict__ m, float* __restrict__ v,
+                                                               AdamK k0, const float* __restrict__ scale) {
+    wb_pdl_enter();
+    const AdamK k = with_device_scale(k0, scale);
+    const int ti = find_tensor(tab, blockIdx.x);
+    const Tensor t = tab.t[ti];
+    if (!t.grad) return;
+    const int64_t len = t.len < 0 ? -t.len : t.len;
+    AdamK kt = k;
+    if (t.len < 0) kt.has_wd = 0;
+    const int64_t at = static_cast<int64_t>(blockIdx.x - tab.first[ti]) * CHUNK, end = min(at + CHUNK, len);
+    for (int64_t i = at + threadIdx.x; i < end; i += THREADS) {
+        float th = t.theta[i], mi = k.first ? 0.f : m[t.offset + i], vi = k.first ? 0.f : v[t.offset + i];
+        adam_one(th, t.grad[i], mi, vi, kt);
+        t.theta[i] = th;
+        m[t.offset + i] = mi;
+        v[t.offset + i] = vi;
+    }
+}
+
+// ---- 8-bit state --------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float decode_m(int c, float unit) { return static_cast<float>(c * abs(c)) * unit; }
+__device__ __forceinline__ float decode_root(int c, float unit) { return static_cast<float>(c * c) * unit; }
+
+// The scale of a block whose largest magnitude has these bits.  One that is not finite poisons the block: its scale is
+// stored as NaN, and every value read from it is NaN.
+__device__ __forceinline__ float block_scale(unsigned int bits) {
+    if (bits >= 0x7f800000u) return __int_as_float(0x7fffffff);
+    return fmaxf(__uint_as_float(bits), TINY);
+}
+__device__ __forceinline__ int encode(float magnitude, float level, float top) {
+    return __float2int_rn(fminf(sqrtf(magnitude * level), top));
+}
+
+template <int N>
+__global__ void __launch_bounds__(THREADS) adam_multi8_kernel(const __grid_constant__ Table<N> tab, int8_t* __restrict__ mc, uint8_t* __restrict__ vc,
+                                                              float* __restrict__ ms, float* __restrict__ vs, AdamK k0,
+                                                              const float* __restrict__ scale) {
+    wb_pdl_enter();
+    const AdamK k = with_device_scale(k0, scale);
+    const int ti = find_tensor(tab, blockIdx.x);
+    const Tensor t = tab.t[ti];
+    if (!t.grad) return;
+    const int64_t len = t.len < 0 ? -t.len : t.len;
+    AdamK kt = k;
+    if (t.len < 0) kt.has_wd = 0;
+    const int lane = threadIdx.x & 31;
+    const int64_t at = static_cast<int64_t>(blockIdx.x - tab.first[ti]) * CHUNK + (threadIdx.x >> 5) * BLOCK8;
+    if (at >= len) return;
+    const int64_t s = t.offset + at, block = s / BLOCK8;
+    const float um = k.first ? 0.f : ms[block] * (1.f / (M_TOP * M_TOP)), ur = k.first ? 0.f : vs[block] * (1.f / (V_TOP * V_TOP));
+    float mn[8], root[8];
+    unsigned int top_m = 0, top_r = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int e = j * 32 + lane;
+        float vi = 0.f;
+        mn[j] = 0.f;
+        root[j] = 0.f;
+        if (at + e < len) {
+            float th = t.theta[at + e];
+            if (!k.first) {
+                mn[j] = decode_m(mc[s + e], um);
+                const float r = decode_root(vc[s + e], ur);
+                vi = r * r;
+            }
+            adam_one(th, t.grad[at + e], mn[j], vi, kt);
+            t.theta[at + e] = th;
+            root[j] = sqrtf(vi);
+        }
+        top_m = max(top_m, __float_as_uint(fabsf(mn[j])));
+        top_r = max(top_r, __float_as_uint(root[j]) & 0x7fffffffu);
+    }
+    const float sm = block_scale(__reduce_max_sync(0xffffffffu, top_m)), sr = block_scale(__reduce_max_sync(0xffffffffu, top_r));
+    const float lm = (M_TOP * M_TOP) / sm, lr = (V_TOP * V_TOP) / sr;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int e = j * 32 + lane;  // behind the tensor's end: the padding, whose codes are 0
+        const int c = encode(fabsf(mn[j]), lm, M_TOP), r = encode(root[j], lr, V_TOP);
+        mc[s + e] = static_cast<int8_t>(mn[j] < 0.f ? -c : c);
+        vc[s + e] = static_cast<uint8_t>(root[j] > 0.f ? max(r, 1) : r);
+    }
+    if (lane == 0) {
+        ms[block] = sm;
+        vs[block] = sr;
+    }
+}
+
+// The values that the 8-bit state stands for.
+__global__ void __launch_bounds__(THREADS) adam_multi8_read_kernel(const int8_t* __restrict__ mc, const uint8_t* __restrict__ vc,
+                                                                   const float* __restrict__ ms, const float* __restrict__ vs, float* __restrict__ m,
+                                                                   float* __restrict__ v, int64_t n) {
+    wb_pdl_enter();
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+    if (i >= n) return;
+    if (m) m[i] = decode_m(mc[i], ms[i / BLOCK8] * (1.f / (M_TOP * M_TOP)));
+    if (v) {
+        const float r = decode_root(vc[i], vs[i / BLOCK8] * (1.f / (V_TOP * V_TOP)));
+        v[i] = r * r;
+    }
+}
+
+// ---- the norm -----------------------------------------------------------------------------------------------
+
+// Squares of f32 are exact in f64 and neither overflow nor vanish there; sums in f64, each in a fixed order.  Block b of
+// this launch takes chunks b, b + gridDim, ... and leaves parts[at + b]; the block that arrives last of all launches
+// joins the `total` parts and leaves the counter zero.
+template <int N>
+__global__ void __launch_bounds__(THREADS) grad_norm_kernel(const __grid_constant__ Table<N> tab, double* __restrict__ parts, int at, int total,
+                                                            unsigned int* __restrict__ counter, double max_norm, float* __restrict__ norm,
+                                                            float* __restrict__ clip) {
+    __shared__ double warp_sum[THREADS / 32];
+    __shared__ unsigned int last;
+    wb_pdl_enter();
+    double acc = 0.0;
+    for (unsigned int c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
+        const int ti = find_tensor(tab, c);
+        const Tensor& t = tab.t[ti];
+        if (!t.grad) continue;
+        const int64_t len = t.len < 0 ? -t.len : t.len, i0 = static_cast<int64_t>(c - tab.first[ti]) * CHUNK, end = min(i0 + CHUNK, len);
+        for (int64_t i = i0 + threadIdx.x; i < end; i += THREADS) {
+            const double g = t.grad[i];
+            acc += g * g;
+        }
+    }
+    auto block_sum = [&](double v) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = v;
+        __syncthreads();
+        double s = 0.0;
+        for (int w = 0; w < THREADS / 32; ++w) s += warp_sum[w];
+        return s;
+    };
+    const double mine = block_sum(acc);
+    if (threadIdx.x == 0) {
+        parts[at + blockIdx.x] = mine;
+        __threadfence();
+        last = atomicAdd(counter, 1u) == static_cast<unsigned int>(total) - 1u;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    acc = 0.0;
+    for (int i = threadIdx.x; i < total; i += THREADS) acc += __ldcg(parts + i);
+    const double sum = sqrt(block_sum(acc));
+    if (threadIdx.x == 0) {
+        *norm = static_cast<float>(sum);
+        if (clip) {
+            const double f = max_norm / (sum + 1e-6);
+            *clip = static_cast<float>(f > 1.0 ? 1.0 : f);  // a NaN stays one
+        }
+        *counter = 0u;
+    }
+}
+
+// ---- the handle ---------------------------------------------------------------------------------------------
+
+constexpr int SMALL = 32, LARGE = 768;  // tensors per launch: 1.2 KB and 28 KB of parameters (limit: 32,764 bytes)
+static_assert(sizeof(Table<LARGE>) + 128 <= 32764, "a launch's parameters");
+
+int64_t padded(int64_t n) { return (n + BLOCK8 - 1) / BLOCK8 * BLOCK8; }
+int64_t chunks_of(int64_t len) { return (len + CHUNK - 1) / CHUNK; }
+
+// All tensors' padded length, or -1.
+int64_t padded_total(const int64_t* lens, int n) {
+    int64_t p = 0;
+    for (int i = 0; i < n; ++i) {
+        if (lens[i] < 0 || lens[i] > (int64_t(1) << 40) - p) return -1;
+        p += padded(lens[i]);
+    }
+    return p;
+}
+int64_t bytes_of(int64_t p, int state_bits) { return state_bits == 32 ? 8 * p : 2 * p + 8 * (p / BLOCK8); }
+
+struct Range {
+    const char *lo, *hi;
+};
+
+}  // namespace
+
+struct WbAdamMulti {
+    WbBackend* b = nullptr;
+    int bits = 32;
+    int64_t padded = 0;
+    char* state = nullptr;
+    bool grads_set = false;
+    std::vector<int64_t> lens, offsets;
+    std::vector<Table<LARGE>> launches;   // the tensors in runs of at most LARGE
+    std::vector<Range> thetas;            // sorted; then the state
+    void* work = nullptr;                 // the norm's counter (16 bytes) and parts
+    size_t work_class = 0;
+    std::vector<int> norm_grids;
+    int norm_parts = 0;
+};
+
+namespace {
+
+template <class F>
+int per_launch(WbAdamMulti* h, F&& launch) {
+    for (size_t l = 0; l < h->launches.size(); ++l) {
+        const Table<LARGE>& t = h->launches[l];
+        if (t.n <= SMALL) {
+            Table<SMALL> s;
+            s.n = t.n;
+            s.chunks = t.chunks;
+            std::copy(t.first, t.first + t.n, s.first);
+            std::copy(t.t, t.t + t.n, s.t);
+            WB_TRY(launch(static_cast<int>(l), s));
+        } else {
+            WB_TRY(launch(static_cast<int>(l), t));
+        }
+    }
+    return WB_OK;
+}
+
+int create(WbBackend* b, const WbAdamTensor* tensors, int n, int state_bits, void* state, int64_t state_bytes, int keep_state, WbAdamMulti* h) {
+    h->b = b;
+    h->bits = state_bits;
+    h->state = static_cast<char*>(state);
+    h->lens.resize(n);
+    for (int i = 0; i < n; ++i) h->lens[i] = tensors[i].len;
+    h->padded = padded_total(h->lens.data(), n);
+    WB_REQUIRE(h->padded >= 0, WB_ERR_INVALID, "wb_adam_multi_create: a length is negative or too large");
+    const int64_t need = bytes_of(h->padded, state_bits);
+    WB_REQUIRE(need == 0 || (state && state_bytes >= need), WB_ERR_INVALID, "wb_adam_multi_create: the state holds %lld bytes, %lld are needed",
+               static_cast<long long>(state ? state_bytes : 0), static_cast<long long>(need));
+    WB_REQUIRE(reinterpret_cast<uintptr_t>(state) % 16 == 0, WB_ERR_INVALID, "wb_adam_multi_create: the state is not aligned to 16 bytes");
+    for (int i = 0; i < n; ++i) {
+        WB_REQUIRE(tensors[i].theta || tensors[i].len == 0, WB_ERR_INVALID, "wb_adam_multi_create: tensor %d is null", i);
+        WB_REQUIRE(reinterpret_cast<uintptr_t>(tensors[i].theta) % 4 == 0, WB_ERR_INVALID, "wb_adam_multi_create: tensor %d is not aligned to 4 bytes", i);
+        if (tensors[i].len == 0) continue;
+        const char* lo = reinterpret_cast<const char*>(tensors[i].theta);
+        h->thetas.push_back({lo, lo + 4 * tensors[i].len});
+    }
+    if (need) h->thetas.push_back({h->state, h->state + need});
+    std::sort(h->thetas.begin(), h->thetas.end(), [](const Range& x, const Range& y) { return x.lo < y.lo; });
+    for (size_t i = 1; i < h->thetas.size(); ++i)
+        WB_REQUIRE(h->thetas[i - 1].hi <= h->thetas[i].lo, WB_ERR_INVALID, "wb_adam_multi_create: two tensors, or a tensor and the state, overlap");
+    int64_t offset = 0;
+    for (int i = 0; i < n; ++i) {
+        h->offsets.push_back(offset);
+        if (h->launches.empty() || h->launches.back().n == LARGE || h->launches.back().chunks + chunks_of(h->lens[i]) > INT32_MAX) {
+            h->launches.emplace_back();
+            h->launches.back().n = 0;
+            h->launches.back().chunks = 0;
+        }
+        Table<LARGE>& t = h->launches.back();
+        t.first[t.n] = t.chunks;
+        t.t[t.n] = {tensors[i].theta, nullptr, offset, tensors[i].no_decay ? -h->lens[i] : h->lens[i]};
+        t.n++;
+        t.chunks += static_cast<unsigned int>(chunks_of(h->lens[i]));
+        offset += padded(h->lens[i]);
+    }
+    for (const auto& t : h->launches) {
+        // at least one block: the norm of nothing is still written
+        const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(t.chunks, 8 * b->sm_count)));
+        h->norm_grids.push_back(grid);
+        h->norm_parts += grid;
+    }
+    WbDeviceGuard dev(b->ordinal);
+    WB_CHECK_CUDA(dev.status);
+    WB_TRY(wb_arena_alloc(b, 16 + sizeof(double) * static_cast<size_t>(h->norm_parts), &h->work, &h->work_class));
+    WB_CHECK_CUDA(cudaMemsetAsync(h->work, 0, 16, b->stream));
+    if (need && !keep_state) WB_CHECK_CUDA(cudaMemsetAsync(state, 0, static_cast<size_t>(need), b->stream));
+    return WB_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t wb_adam_multi_state_bytes(const int64_t* lens, int n, int state_bits) {
+    if (!lens || n < 1 || (state_bits != 32 && state_bits != 8)) return -1;
+    const int64_t p = padded_total(lens, n);
+    return p < 0 ? -1 : bytes_of(p, state_bits);
+}
+
+extern "C" int wb_adam_multi_create(WbBackend* b, const WbAdamTensor* tensors, int n, int state_bits, void* state, int64_t state_bytes, int keep_state,
+                                    WbAdamMulti** out) {
+    WB_REQUIRE(b && tensors && out, WB_ERR_INVALID, "wb_adam_multi_create: null pointer");
+    WB_REQUIRE(n >= 1, WB_ERR_INVALID, "wb_adam_multi_create: no tensors");
+    WB_REQUIRE(state_bits == 32 || state_bits == 8, WB_ERR_UNSUPPORTED, "wb_adam_multi_create: the state has 32 or 8 bits, not %d", state_bits);
+    WbAdamMulti* h = nullptr;
+    int status;
+    try {
+        h = new WbAdamMulti();
+        status = create(b, tensors, n, state_bits, state, state_bytes, keep_state, h);
+    } catch (const std::bad_alloc&) {
+        wb_set_error("wb_adam_multi_create: out of host memory");
+        status = WB_ERR_OOM;
+    }
+    if (status != WB_OK) {
+        wb_adam_multi_destroy(h);
+        return status;
+    }
+    *out = h;
+    return WB_OK;
+}
+
+extern "C" int wb_adam_multi_destroy(WbAdamMulti* h) {
+    if (!h) return WB_OK;
+    if (h->work) wb_arena_free(h->b, h->work, h->work_class);
+    delete h;
+    return WB_OK;
+}
+
+extern "C" int64_t wb_adam_multi_state_len(const WbAdamMulti* h) { return h ? h->padded : -1; }
+
+extern "C" int64_t wb_adam_multi_offset(const WbAdamMulti* h, int index) {
+    return h && index >= 0 && index < static_cast<int>(h->offsets.size()) ? h->offsets[index] : -1;
+}
+
+extern "C" int wb_adam_multi_set_grads(WbAdamMulti* h, const float* const* grads, int n) {
+    WB_REQUIRE(h && grads, WB_ERR_INVALID, "wb_adam_multi_set_grads: null pointer");
+    WB_REQUIRE(n == static_cast<int>(h->lens.size()), WB_ERR_INVALID, "wb_adam_multi_set_grads: %d gradients for %zu tensors", n, h->lens.size());
+    for (int i = 0; i < n; ++i) {
+        if (!grads[i] || h->lens[i] == 0) continue;
+        WB_REQUIRE(reinterpret_cast<uintptr_t>(grads[i]) % 4 == 0, WB_ERR_INVALID, "wb_adam_multi_set_grads: gradient %d is not aligned to 4 bytes", i);
+        const char *lo = reinterpret_cast<const char*>(grads[i]), *hi = lo + 4 * h->lens[i];
+        auto it = std::lower_bound(h->thetas.begin(), h->thetas.end(), hi, [](const Range& r, const char* p) { return r.lo < p; });
+        WB_REQUIRE(it == h->thetas.begin() || (it - 1)->hi <= lo, WB_ERR_INVALID, "wb_adam_multi_set_grads: gradient %d overlaps a parameter or the state", i);
+    }
+    int i = 0;
+    for (auto& t : h->launches)
+        for (int k = 0; k < t.n; ++k) t.t[k].grad = grads[i++];
+    h->grads_set = true;
+    return WB_OK;
+}
+
+extern "C" int wb_adam_multi_grad_norm(WbAdamMulti* h, double max_norm, float* norm, float* clip_scale) {
+    WB_REQUIRE(h && norm, WB_ERR_INVALID, "wb_adam_multi_grad_norm: null pointer");
+    WB_REQUIRE(h->grads_set, WB_ERR_INVALID, "wb_adam_multi_grad_norm: no gradients were set");
+    WB_REQUIRE(!clip_scale || max_norm > 0.0, WB_ERR_INVALID, "wb_adam_multi_grad_norm: the largest norm has to be above 0, got %g", max_norm);
+    WbBackend* b = h->b;
+    WbDeviceGuard dev(b->ordinal);
+    WB_CHECK_CUDA(dev.status);
+    WbProfileScope ps(b, "grad_norm");
+    unsigned int* counter = static_cast<unsigned int*>(h->work);
+    double* parts = reinterpret_cast<double*>(static_cast<char*>(h->work) + 16);
+    int at = 0;
+    return per_launch(h, [&](int l, const auto& tab) -> int {
+        constexpr int N = sizeof(tab.first) / sizeof(tab.first[0]);
+        WB_CHECK_CUDA(wb_launch_pdl(grad_norm_kernel<N>, dim3(h->norm_grids[l]), dim3(THREADS), 0, b->stream, tab, parts, at, h->norm_parts, counter,
+                                    max_norm, norm, clip_scale));
+        WB_LAUNCH_OK(b);
+        at += h->norm_grids[l];
+        return WB_OK;
+    });
+}
+
+extern "C" int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64_t t, double grad_scale, const float* device_grad_scale) {
+    WB_REQUIRE(h && cfg, WB_ERR_INVALID, "wb_adam_multi_step: null pointer");
+    WB_REQUIRE(h->grads_set, WB_ERR_INVALID, "wb_adam_multi_step: no gradients were set");
+    WB_REQUIRE(t >= 1 && t <= INT32_MAX, WB_ERR_INVALID, "wb_adam_multi_step: step counts from 1 to 2^31 - 1");
+    WbBackend* b = h->b;
+    WbDeviceGuard dev(b->ordinal);
+    WB_CHECK_CUDA(dev.status);
+    WbProfileScope ps(b, h->bits == 32 ? "adam_multi" : "adam_multi_8bit");
+    const AdamK k = wb_adam_constants(t, cfg->lr, cfg->beta1, cfg->beta2, cfg->eps, cfg->weight_decay, cfg->decoupled, grad_scale);
+    const int64_t p = h->padded;
+    return per_launch(h, [&](int, const auto& tab) -> int {
+        constexpr int N = sizeof(tab.first) / sizeof(tab.first[0]);
+        if (tab.chunks == 0) return WB_OK;
+        if (h->bits == 32) {
+            float* m = reinterpret_cast<float*>(h->state);
+            WB_CHECK_CUDA(wb_launch_pdl(adam_multi32_kernel<N>, dim3(tab.chunks), dim3(THREADS), 0, b->stream, tab, m, m + p, k, device_grad_scale));
+        } else {
+            float* scales = reinterpret_cast<float*>(h->state + 2 * p);
+            WB_CHECK_CUDA(wb_launch_pdl(adam_multi8_kernel<N>, dim3(tab.chunks), dim3(THREADS), 0, b->stream, tab, reinterpret_cast<int8_t*>(h->state),
+                                        reinterpret_cast<uint8_t*>(h->state + p), scales, scales + p / BLOCK8, k, device_grad_scale));
+        }
+        WB_LAUNCH_OK(b);
+        return WB_OK;
+    });
+}
+
+extern "C" int wb_adam_multi_read_state(WbAdamMulti* h, float* m, float* v) {
+    WB_REQUIRE(h && (m || v), WB_ERR_INVALID, "wb_adam_multi_read_state: null pointer");
+    if (h->padded == 0) return WB_OK;
+    WbBackend* b = h->b;
+    const int64_t p = h->padded;
+    const char* state = h->state;
+    const WbSpan spans[3] = {{state, state + bytes_of(p, h->bits), false},
+                             {reinterpret_cast<char*>(m), reinterpret_cast<char*>(m) + (m ? 4 * p : 0), true},
+                             {reinterpret_cast<char*>(v), reinterpret_cast<char*>(v) + (v ? 4 * p : 0), true}};
+    WB_REQUIRE(!wb_spans_clash(spans, 3), WB_ERR_INVALID, "wb_adam_multi_read_state: the outputs overlap each other or the state");
+    WB_REQUIRE((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) % 4 == 0, WB_ERR_INVALID,
+               "wb_adam_multi_read_state: an output is not aligned to 4 bytes");
+    WbDeviceGuard dev(b->ordinal);
+    WB_CHECK_CUDA(dev.status);
+    WbProfileScope ps(b, "adam_multi_read_state");
+    if (h->bits == 32) {
+        if (m) WB_CHECK_CUDA(cudaMemcpyAsync(m, state, static_cast<size_t>(4 * p), cudaMemcpyDeviceToDevice, b->stream));
+        if (v) WB_CHECK_CUDA(cudaMemcpyAsync(v, state + 4 * p, static_cast<size_t>(4 * p), cudaMemcpyDeviceToDevice, b->stream));
+        return WB_OK;
+    }
+    const float* scales = reinterpret_cast<const float*>(state + 2 * p);
+    const int64_t grid = (p + THREADS - 1) / THREADS;
+    WB_REQUIRE(grid <= INT32_MAX, WB_ERR_INVALID, "wb_adam_multi_read_state: state too large");
+    WB_CHECK_CUDA(wb_launch_pdl(adam_multi8_read_kernel, dim3(static_cast<unsigned>(grid)), dim3(THREADS), 0, b->stream,
+                                reinterpret_cast<const int8_t*>(state), reinterpret_cast<const uint8_t*>(state + p), scales, scales + p / BLOCK8, m, v, p));
+    WB_LAUNCH_OK(b);
+    return WB_OK;
+}

@@ -148,6 +148,33 @@ struct WbProfileScope {
     }
 };
 
+// Makes the backend's device the calling thread's current one for the length of an entry point.
+struct WbDeviceGuard {
+    int before = -1;
+    cudaError_t status;
+    explicit WbDeviceGuard(int ordinal) {
+        status = cudaGetDevice(&before);
+        if (status == cudaSuccess && before != ordinal) status = cudaSetDevice(ordinal);
+        else before = -1;
+    }
+    ~WbDeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// Bytes [lo, hi) that an entry point reads or writes.  True if two of them meet and at least one is written.
+struct WbSpan {
+    const char* lo;
+    const char* hi;
+    bool written;
+};
+inline bool wb_spans_clash(const WbSpan* s, int n) {
+    for (int i = 0; i < n; ++i)
+        for (int j = i + 1; j < n; ++j)
+            if ((s[i].written || s[j].written) && s[i].lo < s[j].hi && s[j].lo < s[i].hi) return true;
+    return false;
+}
+
 // ---- iteration plans for element-wise kernels ---------------------------------------------------
 // The output of every element-wise op is contiguous; the plan describes how up to three operand
 // views walk alongside it after size-1 dims are dropped and mergeable neighbours are fused.
