@@ -102,6 +102,262 @@ __global__ void __launch_bounds__(THREADS) ln_dx_any_kernel(const T* __restrict_
     }
 }
 
+// ---- rows of unit stride ---------------------------------------------------------------------------------
+// TPR threads hold one row in registers: vector j of thread t covers columns (j TPR + t) VEC ..., so every access of a
+// warp is one contiguous run.  Rows are `pitch` elements apart.
+
+template <class T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+
+template <class T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
+    return *reinterpret_cast<const Pack<T, VEC>*>(p);
+}
+
+// Sum over the TPR threads of a row, returned to all of them.  Rows of more than a warp meet at the barrier of their
+// group (`bar`, at least 1) and join the warps' sums, `part` (2 K warps), in a second tree; two buffers in turn make one
+// barrier per sum enough.
+template <class T, int TPR, int K>
+__device__ __forceinline__ void row_sum(T (&v)[K], T* part, int bar, unsigned int& turn) {
+#pragma unroll
+    for (int d = (TPR < 32 ? TPR : 32) / 2; d > 0; d >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], d);
+    if constexpr (TPR > 32) {
+        constexpr int W = TPR / 32;
+        const int lane = threadIdx.x & 31, warp = threadIdx.x % TPR >> 5;
+        T* mine = part + (turn & 1) * K * W;
+        ++turn;
+        if (lane == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) mine[k * W + warp] = v[k];
+        asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(TPR) : "memory");
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            T s = mine[k * W + lane % W];
+#pragma unroll
+            for (int d = W / 2; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+            v[k] = s;
+        }
+    }
+}
+
+template <int TPR>
+constexpr int fwd_threads = TPR < 128 ? 128 : TPR;
+
+template <class T, int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* __restrict__ x, int64_t pitch, int64_t rows, int cols,
+                                                                       const T* __restrict__ w, const T* __restrict__ bias, T eps, T inv_cols,
+                                                                       T* __restrict__ y, T* __restrict__ mean_out, T* __restrict__ rstd_out) {
+    constexpr int G = fwd_threads<TPR> / TPR;
+    __shared__ T part[G][TPR > 32 ? 2 * TPR / 32 : 1];
+    wb_pdl_enter();
+    const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * G + group;
+    const bool live = row < rows;  // the other rows of a warp still need this one in their shuffles
+    if (TPR >= 32 && !live) return;
+    const T* xr = x + row * pitch;
+    Pack<T, VEC> a[NV];
+    T s[1] = {0};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + t) * VEC;
+        if (live && c < cols) a[j] = load_pack<T, VEC>(xr + c);
+        else
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) a[j].v[i] = 0;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[0] += a[j].v[i];
+    }
+    unsigned int turn = 0;
+    row_sum<T, TPR, 1>(s, part[group], 1 + group, turn);
+    const T mean = s[0] * inv_cols;
+    T q[1] = {0};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const bool in = (j * TPR + t) * VEC < cols;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            a[j].v[i] -= mean;
+            if (in) q[0] += a[j].v[i] * a[j].v[i];
+        }
+    }
+    row_sum<T, TPR, 1>(q, part[group], 1 + group, turn);
+    const T rstd = T(1) / sqrt(q[0] * inv_cols + eps);
+    if (!live) return;
+    T* yr = y + row * cols;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + t) * VEC;
+        if (c < cols) {
+            Pack<T, VEC> o, pw, pb;
+            if (w) pw = load_pack<T, VEC>(w + c);
+            if (bias) pb = load_pack<T, VEC>(bias + c);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                o.v[i] = a[j].v[i] * rstd;
+                if (w) o.v[i] *= pw.v[i];
+                if (bias) o.v[i] += pb.v[i];
+            }
+            *reinterpret_cast<Pack<T, VEC>*>(yr + c) = o;
+        }
+    }
+    if (t == 0) {
+        if (mean_out) mean_out[row] = mean;
+        if (rstd_out) rstd_out[row] = rstd;
+    }
+}
+
+// Backward.  A group of TPR threads walks rows id, id + groups, ...; the rows ahead are fetched by cp.async into a ring of
+// DEPTH slots in shared memory.  A thread reads back only what it copied itself, so the ring needs no barrier.  The
+// weight's and the bias's gradients of its columns stay in the thread's registers over all its rows; at the end the groups
+// of a block are joined in shared memory and the block leaves one row of partials.
+constexpr int BWD_THREADS = 256;
+
+__device__ __forceinline__ void async_copy(void* smem, const void* gmem, std::integral_constant<int, 16>) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void async_copy(void* smem, const void* gmem, std::integral_constant<int, 8>) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void async_copy(void* smem, const void* gmem, std::integral_constant<int, 4>) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "l"(gmem) : "memory");
+}
+
+template <int TPR>
+constexpr int bwd_threads = TPR < BWD_THREADS ? BWD_THREADS : TPR;
+
+template <class T, int VEC, int TPR, int NV, int DEPTH>
+__global__ void __launch_bounds__(bwd_threads<TPR>) ln_bwd_rows_kernel(const T* __restrict__ x, int64_t pitch_x, const T* __restrict__ dy, int64_t pitch_g,
+                                                                       int64_t rows, int cols, const T* __restrict__ w, const T* __restrict__ mean,
+                                                                       const T* __restrict__ rstd, T inv_cols, T* __restrict__ dx,
+                                                                       T* __restrict__ parts) {
+    constexpr int THREADS_B = bwd_threads<TPR>, G = THREADS_B / TPR, E = NV * VEC;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    Pack<T, VEC>* ring = reinterpret_cast<Pack<T, VEC>*>(smem_raw);  // [DEPTH][2][NV][THREADS_B]
+    __shared__ T part[G][TPR > 32 ? 4 * TPR / 32 : 1];
+    wb_pdl_enter();
+    const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+    const int64_t groups = static_cast<int64_t>(gridDim.x) * G, first = static_cast<int64_t>(blockIdx.x) * G + group;
+    auto slot = [&](int stage, int which, int j) -> Pack<T, VEC>& { return ring[((stage * 2 + which) * NV + j) * THREADS_B + threadIdx.x]; };
+    T wv[E], aw[E], ab[E];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int c = (j * TPR + t) * VEC + i;
+            wv[j * VEC + i] = c < cols ? (w ? w[c] : T(1)) : T(0);
+            aw[j * VEC + i] = ab[j * VEC + i] = 0;
+            // columns behind the row's end: their slots are never copied to and stay 0
+            for (int d = 0; d < DEPTH; ++d) slot(d, 0, j).v[i] = slot(d, 1, j).v[i] = 0;
+        }
+    auto fetch = [&](int64_t row, int stage) {
+        if (row < rows) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = (j * TPR + t) * VEC;
+                if (c < cols) {
+                    async_copy(&slot(stage, 0, j), x + row * pitch_x + c, std::integral_constant<int, sizeof(T) * VEC>{});
+                    async_copy(&slot(stage, 1, j), dy + row * pitch_g + c, std::integral_constant<int, sizeof(T) * VEC>{});
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) fetch(first + d * groups, d);
+    T mu = 0, rs = 0;
+    if (first < rows) {
+        mu = mean[first];
+        rs = rstd[first];
+    }
+    unsigned int turn = 0;
+    int stage = 0;
+    // groups narrower than a warp share its shuffles: they all walk as far as the warp's first one
+    const int64_t lead = TPR < 32 ? first - group % (32 / (TPR < 32 ? TPR : 32)) : first;
+    for (int64_t row = first, at = lead; at < rows; row += groups, at += groups) {
+        fetch(row + (DEPTH - 1) * groups, stage == 0 ? DEPTH - 1 : stage - 1);
+        T mu_next = 0, rs_next = 0;
+        if (row + groups < rows) {
+            mu_next = mean[row + groups];
+            rs_next = rstd[row + groups];
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+        const bool live = TPR >= 32 || row < rows;
+        T xh[E], g[E], s[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const Pack<T, VEC> px = slot(stage, 0, j), pg = slot(stage, 1, j);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int e = j * VEC + i;
+                const T up = live ? pg.v[i] : T(0);
+                xh[e] = live ? (px.v[i] - mu) * rs : T(0);  // not live: the slot holds an older row
+                aw[e] += up * xh[e];
+                ab[e] += up;
+                g[e] = up * wv[e];
+                s[0] += g[e];
+                s[1] += g[e] * xh[e];
+            }
+        }
+        if (dx) {
+            row_sum<T, TPR, 2>(s, part[group], 1 + group, turn);
+            const T c0 = s[0] * inv_cols, c1 = s[1] * inv_cols;
+            if (live) {
+                T* dr = dx + row * cols;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int c = (j * TPR + t) * VEC;
+                    Pack<T, VEC> o;
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) o.v[i] = rs * (g[j * VEC + i] - c0 - xh[j * VEC + i] * c1);
+                    if (c < cols) *reinterpret_cast<Pack<T, VEC>*>(dr + c) = o;
+                }
+            }
+        }
+        mu = mu_next;
+        rs = rs_next;
+        stage = stage + 1 == DEPTH ? 0 : stage + 1;
+    }
+    if (!parts) return;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (G > 1) {  // the groups' sums, in the groups' order
+        T* joined = reinterpret_cast<T*>(smem_raw);  // [2][G][TPR E]
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int c = (j * TPR + t) * VEC + i;
+                joined[group * TPR * E + c] = aw[j * VEC + i];
+                joined[(G + group) * TPR * E + c] = ab[j * VEC + i];
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < cols; c += THREADS_B) {
+            T sw = joined[c], sb = joined[G * TPR * E + c];
+            for (int k = 1; k < G; ++k) {
+                sw += joined[k * TPR * E + c];
+                sb += joined[(G + k) * TPR * E + c];
+            }
+            parts[static_cast<int64_t>(blockIdx.x) * cols + c] = sw;
+            parts[static_cast<int64_t>(gridDim.x + blockIdx.x) * cols + c] = sb;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int c = (j * TPR + t) * VEC + i;
+                if (c < cols) {
+                    parts[static_cast<int64_t>(blockIdx.x) * cols + c] = aw[j * VEC + i];
+                    parts[static_cast<int64_t>(gridDim.x + blockIdx.x) * cols + c] = ab[j * VEC + i];
+                }
+            }
+    }
+}
+
 // dw and db of 32 columns over one slab of rows: partials [2][slabs][cols].
 template <class T>
 __global__ void __launch_bounds__(THREADS) ln_dw_any_kernel(const T* __restrict__ x, RowView vx, const T* __restrict__ dy, RowView vg, int64_t rows,
@@ -137,20 +393,28 @@ __global__ void __launch_bounds__(THREADS) ln_dw_any_kernel(const T* __restrict_
     }
 }
 
-// Sums the slabs of both partial arrays in order.
+// Sums the slabs of both partial arrays: 32 columns per block, eight runs of slabs side by side, joined in order.
 template <class T>
 __global__ void __launch_bounds__(THREADS) ln_dw_join_kernel(const T* __restrict__ parts, int slabs, int64_t cols, T* __restrict__ dw,
                                                              T* __restrict__ db) {
+    __shared__ double sum[THREADS / 32][32];
     wb_pdl_enter();
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
-    if (c >= cols) return;
-    double aw = 0.0, ab = 0.0;
-    for (int k = 0; k < slabs; ++k) {
-        aw += parts[static_cast<int64_t>(k) * cols + c];
-        ab += parts[static_cast<int64_t>(slabs + k) * cols + c];
+    T* out = blockIdx.y == 0 ? dw : db;
+    if (!out) return;
+    const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+    const T* p = parts + static_cast<int64_t>(blockIdx.y) * slabs * cols;
+    double acc = 0.0;
+    if (c < cols) {
+#pragma unroll 8
+        for (int k = line; k < slabs; k += THREADS / 32) acc += p[static_cast<int64_t>(k) * cols + c];
     }
-    if (dw) dw[c] = static_cast<T>(aw);
-    if (db) db[c] = static_cast<T>(ab);
+    sum[line][lane] = acc;
+    __syncthreads();
+    if (line == 0 && c < cols) {
+        for (int k = 1; k < THREADS / 32; ++k) acc += sum[k][lane];
+        out[c] = static_cast<T>(acc);
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
@@ -242,14 +506,96 @@ struct SpanList {
 // Rows are summed in at most this many slabs for the weight's gradient.
 int dw_slabs(int sm_count, int64_t rows) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 2 * sm_count))); }
 
+// Unit stride along the row and one stride from row to row.
+bool plain_rows(const RowView& v, const Shape& s) { return v.nd_row == 1 && v.nd_col == 1 && (v.st_col[0] == 1 || s.cols == 1); }
+
+// 16-byte accesses: every row of every operand starts on a 16-byte boundary.
+template <class T>
+constexpr int wide = 16 / static_cast<int>(sizeof(T));
+template <class T>
+bool rows_aligned(const void* p, int64_t pitch, int64_t cols) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch % wide<T> == 0 && cols % wide<T> == 0;
+}
+
+// Calls f with (threads per row, vectors per thread) for rows of `packs` vectors, at most MOST vectors per thread: the
+// fewest threads that hold the row, so that small rows share a block and the reductions stay short.
+template <int MOST, class F>
+bool choose_row(int64_t packs, F&& f) {
+    auto per = [&](auto tpr) -> bool {
+        constexpr int TPR = decltype(tpr)::value;
+        if (packs > static_cast<int64_t>(TPR) * MOST) return false;
+        const int64_t nv = (packs + TPR - 1) / TPR;
+        if constexpr (TPR == 8) {
+            if (nv <= 1) return f(tpr, std::integral_constant<int, 1>{}), true;
+            if (nv <= 2) return f(tpr, std::integral_constant<int, 2>{}), true;
+        }
+        if constexpr (TPR == 8 && MOST > 4)
+            if (nv <= MOST / 4) return f(tpr, std::integral_constant<int, MOST / 4>{}), true;
+        if constexpr (TPR == 8)
+            if (nv <= MOST / 2) return f(tpr, std::integral_constant<int, MOST / 2>{}), true;
+        if (nv <= MOST * 3 / 4) return f(tpr, std::integral_constant<int, MOST * 3 / 4>{}), true;
+        return f(tpr, std::integral_constant<int, MOST>{}), true;
+    };
+    return per(std::integral_constant<int, 8>{}) || per(std::integral_constant<int, 16>{}) || per(std::integral_constant<int, 32>{}) ||
+           per(std::integral_constant<int, 64>{}) || per(std::integral_constant<int, 128>{}) || per(std::integral_constant<int, 256>{}) ||
+           per(std::integral_constant<int, 512>{}) || per(std::integral_constant<int, 1024>{});
+}
+
+template <class T>
+constexpr int row_elems = 64 / static_cast<int>(sizeof(T));  // elements of a row that a thread holds at most
+
+template <class T, int VEC>
+bool fwd_rows(WbBackend* b, const T* x, int64_t pitch, const Shape& s, const T* w, const T* bias, double eps, T* y, T* mean, T* rstd, cudaError_t* err) {
+    return choose_row<row_elems<T> / VEC>((s.cols + VEC - 1) / VEC, [&](auto tpr, auto nv) {
+        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, G = fwd_threads<TPR> / TPR;
+        const int64_t grid = (s.rows + G - 1) / G;
+        if (grid > INT32_MAX) {
+            *err = cudaErrorInvalidConfiguration;
+            return;
+        }
+        *err = wb_launch_pdl(ln_fwd_rows_kernel<T, VEC, TPR, NV>, dim3(static_cast<unsigned>(grid)), dim3(fwd_threads<TPR>), 0, b->stream, x, pitch,
+                             s.rows, static_cast<int>(s.cols), w, bias, static_cast<T>(eps), static_cast<T>(1.0 / static_cast<double>(s.cols)), y, mean,
+                             rstd);
+    });
+}
+
 template <class T>
 int fwd_typed(WbBackend* b, const WbView* x, int nd, const Shape& s, const T* w, const T* bias, double eps, T* y, T* mean, T* rstd) {
     const T* xp = reinterpret_cast<const T*>(view_data(*x));
     const RowView vx = row_view(*x, nd);
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(s.rows, 65535));
-    WB_CHECK_CUDA(wb_launch_pdl(ln_fwd_any_kernel<T>, dim3(grid), dim3(THREADS), 0, b->stream, xp, vx, s.rows, s.cols, w, bias, eps, y, mean, rstd));
+    cudaError_t err = cudaSuccess;
+    bool done = false;
+    if (plain_rows(vx, s)) {
+        const int64_t pitch = vx.st_row[0];
+        if (rows_aligned<T>(xp, pitch, s.cols) && rows_aligned<T>(y, s.cols, s.cols) &&
+            ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(bias)) & 15) == 0)
+            done = fwd_rows<T, wide<T>>(b, xp, pitch, s, w, bias, eps, y, mean, rstd, &err);
+        else
+            done = fwd_rows<T, 1>(b, xp, pitch, s, w, bias, eps, y, mean, rstd, &err);
+    }
+    if (!done) {
+        const unsigned grid = static_cast<unsigned>(std::min<int64_t>(s.rows, 65535));
+        err = wb_launch_pdl(ln_fwd_any_kernel<T>, dim3(grid), dim3(THREADS), 0, b->stream, xp, vx, s.rows, s.cols, w, bias, eps, y, mean, rstd);
+    }
+    WB_CHECK_CUDA(err);
     WB_LAUNCH_OK(b);
     return WB_OK;
+}
+
+template <class T, int VEC>
+bool bwd_rows(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t pitch_g, const Shape& s, const T* w, const T* mean, const T* rstd, T* dx,
+              T* parts, int* slabs, cudaError_t* err) {
+    return choose_row<row_elems<T> / VEC>((s.cols + VEC - 1) / VEC, [&](auto tpr, auto nv) {
+        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, N = bwd_threads<TPR>, G = N / TPR, DEPTH = TPR > 512 ? 1 : 2;
+        constexpr size_t smem = sizeof(T) * 2 * DEPTH * NV * VEC * N;
+        static_assert(smem <= 200 * 1024, "ring");
+        auto kernel = ln_bwd_rows_kernel<T, VEC, TPR, NV, DEPTH>;
+        *err = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (*err != cudaSuccess) return;
+        *slabs = static_cast<int>(std::min<int64_t>(dw_slabs(b->sm_count, s.rows), (s.rows + G - 1) / G));
+        *err = wb_launch_pdl(kernel, dim3(*slabs), dim3(N), smem, b->stream, x, pitch_x, dy, pitch_g, s.rows, static_cast<int>(s.cols), w, mean, rstd,
+                             static_cast<T>(1.0 / static_cast<double>(s.cols)), dx, parts);
+    });
 }
 
 template <class T>
@@ -258,21 +604,38 @@ int bwd_typed(WbBackend* b, const WbView* x, const WbView* dy, int nd, const Sha
     const T* xp = reinterpret_cast<const T*>(view_data(*x));
     const T* gp = reinterpret_cast<const T*>(view_data(*dy));
     const RowView vx = row_view(*x, nd), vg = row_view(*dy, nd);
-    if (dx) {
+    const bool sums = dw || db;
+    if (!dx && !sums) return WB_OK;
+    cudaError_t err = cudaSuccess;
+    bool done = false;
+    int slabs = dw_slabs(b->sm_count, s.rows);
+    if (plain_rows(vx, s) && plain_rows(vg, s)) {
+        const int64_t px = vx.st_row[0], pg = vg.st_row[0];
+        T* to = sums ? parts : nullptr;
+        if (rows_aligned<T>(xp, px, s.cols) && rows_aligned<T>(gp, pg, s.cols) && rows_aligned<T>(dx, s.cols, s.cols))
+            done = bwd_rows<T, wide<T>>(b, xp, px, gp, pg, s, w, mean, rstd, dx, to, &slabs, &err);
+        else
+            done = bwd_rows<T, 1>(b, xp, px, gp, pg, s, w, mean, rstd, dx, to, &slabs, &err);
+        if (done) {
+            WB_CHECK_CUDA(err);
+            WB_LAUNCH_OK(b);
+        }
+    }
+    if (!done && dx) {
         const unsigned grid = static_cast<unsigned>(std::min<int64_t>(s.rows, 65535));
         WB_CHECK_CUDA(wb_launch_pdl(ln_dx_any_kernel<T>, dim3(grid), dim3(THREADS), 0, b->stream, xp, vx, gp, vg, s.rows, s.cols, w, mean, rstd, dx));
         WB_LAUNCH_OK(b);
     }
-    if (dw || db) {
-        const int slabs = dw_slabs(b->sm_count, s.rows);
+    if (!sums) return WB_OK;
+    if (!done) {
         const unsigned strips = static_cast<unsigned>(std::min<int64_t>((s.cols + 31) / 32, 65535));
         WB_CHECK_CUDA(wb_launch_pdl(ln_dw_any_kernel<T>, dim3(strips, slabs), dim3(THREADS), 0, b->stream, xp, vx, gp, vg, s.rows, s.cols, mean, rstd,
                                     parts, slabs));
         WB_LAUNCH_OK(b);
-        WB_CHECK_CUDA(wb_launch_pdl(ln_dw_join_kernel<T>, dim3(static_cast<unsigned>((s.cols + THREADS - 1) / THREADS)), dim3(THREADS), 0, b->stream,
-                                    static_cast<const T*>(parts), slabs, s.cols, dw, db));
-        WB_LAUNCH_OK(b);
     }
+    WB_CHECK_CUDA(wb_launch_pdl(ln_dw_join_kernel<T>, dim3(static_cast<unsigned>((s.cols + 31) / 32), 2), dim3(THREADS), 0, b->stream,
+                                static_cast<const T*>(parts), slabs, s.cols, dw, db));
+    WB_LAUNCH_OK(b);
     return WB_OK;
 }
 
