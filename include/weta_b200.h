@@ -184,7 +184,7 @@ double wb_host_normal_sample(uint64_t seed, uint64_t i, double mean, double std)
 
 /* ==== extension: entry points with no trait method today ===================================== */
 
-/* Reads the device-side flag a tensor-core kernel raises when one of its bounded barrier waits
+/* Reads the device-side flag a tensor-core kernel (or the layer norm's) raises when one of its bounded barrier waits
  * runs out (WB_ERR_TIMEOUT), then clears it.  Synchronises the stream.  The reference has no
  * counterpart: cuBLAS reports its own failures through the call's status (lib.rs:387). */
 int wb_gemm_check(WbBackend* b);

@@ -42,6 +42,8 @@ int wb_conv3_dgrad(WbBackend* b, const WbConv3& g, const float* const dy3[3], co
 int wb_tc_encode(WbBackend* be, const float* ptr, const uint64_t dims[3], const uint64_t strides[2], const uint32_t box[3], bool swizzle128,
                  CUtensorMap* map);
 int wb_tc_error_flag(WbBackend* be, int** flag);
+// The flag of layer_norm.cu's bounded waits (a part of wb_gemm_check).
+int wb_layer_norm_check(WbBackend* b);
 
 // BatchNorm+ReLU+pool backward of the first convolution block fused with that convolution's weight gradient
 // (conv1_bwd_fused.cu): dconv is never written.  `cols` is the block's im2col matrix [n][ck][h*w].

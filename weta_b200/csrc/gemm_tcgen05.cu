@@ -606,6 +606,7 @@ extern "C" int wb_gemm_selftest_timeout(WbBackend* b, int polls) {
 // Reads the device-side error flag the GEMM kernels raise when a bounded wait runs out.
 // Synchronises the stream; meant for tests and for wb_synchronize-style checkpoints.
 extern "C" int wb_gemm_check(WbBackend* b) {
+    WB_TRY(wb_layer_norm_check(b));
     if (!b->gemm_state) return WB_OK;
     GemmState* st = static_cast<GemmState*>(b->gemm_state);
     WB_CHECK_CUDA(cudaMemcpyAsync(st->error_host, st->error_flag, sizeof(int), cudaMemcpyDeviceToHost, b->stream));

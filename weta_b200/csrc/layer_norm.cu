@@ -117,10 +117,14 @@ __device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
 }
 
 // Sum over the TPR threads of a row, returned to all of them.  Rows of more than a warp meet at the barrier of their
-// group (`bar`, at least 1) and join the warps' sums, `part` (2 K warps), in a second tree; two buffers in turn make one
-// barrier per sum enough.
-template <class T, int TPR, int K>
-__device__ __forceinline__ void row_sum(T (&v)[K], T* part, int bar, unsigned int& turn) {
+// group (`bar`, at least 1; the block's own where it is one group: a barrier known only at run time reserves all sixteen,
+// which let four blocks onto an SM) and join the warps' sums, `part` (2 K warps), in a second tree; two buffers in turn make one
+// barrier per sum enough.  `after_barrier` runs there.
+struct Nothing {
+    __device__ __forceinline__ void operator()() const {}
+};
+template <class T, int TPR, int G, int K, class F = Nothing>
+__device__ __forceinline__ void row_sum(T (&v)[K], T* part, int bar, unsigned int& turn, F&& after_barrier = F()) {
 #pragma unroll
     for (int d = (TPR < 32 ? TPR : 32) / 2; d > 0; d >>= 1)
 #pragma unroll
@@ -133,7 +137,9 @@ __device__ __forceinline__ void row_sum(T (&v)[K], T* part, int bar, unsigned in
         if (lane == 0)
 #pragma unroll
             for (int k = 0; k < K; ++k) mine[k * W + warp] = v[k];
-        asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(TPR) : "memory");
+        if constexpr (G == 1) __syncthreads();
+        else asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(TPR) : "memory");
+        after_barrier();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             T s = mine[k * W + lane % W];
@@ -145,7 +151,7 @@ __device__ __forceinline__ void row_sum(T (&v)[K], T* part, int bar, unsigned in
 }
 
 template <int TPR>
-constexpr int fwd_threads = TPR < 128 ? 128 : TPR;
+constexpr int fwd_threads = TPR < 64 ? 128 : TPR;
 
 template <class T, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* __restrict__ x, int64_t pitch, int64_t rows, int cols,
@@ -172,7 +178,7 @@ __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* 
         for (int i = 0; i < VEC; ++i) s[0] += a[j].v[i];
     }
     unsigned int turn = 0;
-    row_sum<T, TPR, 1>(s, part[group], 1 + group, turn);
+    row_sum<T, TPR, G, 1>(s, part[group], 1 + group, turn);
     const T mean = s[0] * inv_cols;
     T q[1] = {0};
 #pragma unroll
@@ -184,7 +190,7 @@ __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* 
             if (in) q[0] += a[j].v[i] * a[j].v[i];
         }
     }
-    row_sum<T, TPR, 1>(q, part[group], 1 + group, turn);
+    row_sum<T, TPR, G, 1>(q, part[group], 1 + group, turn);
     const T rstd = T(1) / sqrt(q[0] * inv_cols + eps);
     if (!live) return;
     T* yr = y + row * cols;
@@ -210,151 +216,439 @@ __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* 
     }
 }
 
-// Backward.  A group of TPR threads walks rows id, id + groups, ...; the rows ahead are fetched by cp.async into a ring of
-// DEPTH slots in shared memory.  A thread reads back only what it copied itself, so the ring needs no barrier.  The
-// weight's and the bias's gradients of its columns stay in the thread's registers over all its rows; at the end the groups
-// of a block are joined in shared memory and the block leaves one row of partials.
-constexpr int BWD_THREADS = 256;
-
-__device__ __forceinline__ void async_copy(void* smem, const void* gmem, std::integral_constant<int, 16>) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "l"(gmem) : "memory");
+// ---- two values at a time --------------------------------------------------------------------------------
+// sm_100 has packed f32 arithmetic (two IEEE operations per instruction and lane); f64 stays scalar.
+template <class T>
+struct Pair;
+template <>
+struct Pair<float> {
+    uint64_t v;
+};
+template <>
+struct Pair<double> {
+    double a, b;
+};
+__device__ __forceinline__ Pair<float> pair(float a, float b) {
+    Pair<float> r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
 }
-__device__ __forceinline__ void async_copy(void* smem, const void* gmem, std::integral_constant<int, 8>) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "l"(gmem) : "memory");
+__device__ __forceinline__ Pair<double> pair(double a, double b) { return {a, b}; }
+__device__ __forceinline__ void unpair(const Pair<float>& p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ void unpair(const Pair<double>& p, double& a, double& b) {
+    a = p.a;
+    b = p.b;
 }
-__device__ __forceinline__ void async_copy(void* smem, const void* gmem, std::integral_constant<int, 4>) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "l"(gmem) : "memory");
+__device__ __forceinline__ Pair<float> operator+(const Pair<float>& x, const Pair<float>& y) {
+    Pair<float> r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(x.v), "l"(y.v));
+    return r;
+}
+__device__ __forceinline__ Pair<float> operator*(const Pair<float>& x, const Pair<float>& y) {
+    Pair<float> r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(x.v), "l"(y.v));
+    return r;
+}
+__device__ __forceinline__ Pair<float> muladd(const Pair<float>& x, const Pair<float>& y, const Pair<float>& z) {
+    Pair<float> r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(x.v), "l"(y.v), "l"(z.v));
+    return r;
+}
+__device__ __forceinline__ Pair<double> operator+(const Pair<double>& x, const Pair<double>& y) { return {x.a + y.a, x.b + y.b}; }
+__device__ __forceinline__ Pair<double> operator*(const Pair<double>& x, const Pair<double>& y) { return {x.a * y.a, x.b * y.b}; }
+__device__ __forceinline__ Pair<double> muladd(const Pair<double>& x, const Pair<double>& y, const Pair<double>& z) {
+    return {fma(x.a, y.a, z.a), fma(x.b, y.b, z.b)};
 }
 
-template <int TPR>
-constexpr int bwd_threads = TPR < BWD_THREADS ? BWD_THREADS : TPR;
+// ---- rows through a ring in shared memory --------------------------------------------------------------------
+// A group of threads walks spans: R rows that follow each other in memory (one row, or a part of it, where they do not).
+// The spans ahead are fetched into a ring of two to four slots by one bulk copy for each operand, which costs the group one
+// thread's instruction whatever the width.  A bulk copy takes whole 16-byte units; the elements short of a unit at either
+// end of a span, and the rows' statistics, are copied beside it one by one (cp.async) by lanes of the group, so nothing
+// outside the span is read.
+constexpr int MOST_RING = 4;
+constexpr uint32_t POLLS = 1u << 26;
+__device__ int g_ln_timeout;  // raised when a bounded wait runs out; read by wb_layer_norm_check
 
-template <class T, int VEC, int TPR, int NV, int DEPTH>
-__global__ void __launch_bounds__(bwd_threads<TPR>) ln_bwd_rows_kernel(const T* __restrict__ x, int64_t pitch_x, const T* __restrict__ dy, int64_t pitch_g,
-                                                                       int64_t rows, int cols, const T* __restrict__ w, const T* __restrict__ mean,
-                                                                       const T* __restrict__ rstd, T inv_cols, T* __restrict__ dx,
-                                                                       T* __restrict__ parts) {
-    constexpr int THREADS_B = bwd_threads<TPR>, G = THREADS_B / TPR, E = NV * VEC;
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void bar_init(uint64_t* bar) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(bar)));
+}
+__device__ __forceinline__ void bar_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes),
+                 "r"(smem_addr(bar))
+                 : "memory");
+}
+template <class T>
+__device__ __forceinline__ void copy_one(T* dst, const T* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(dst)), "l"(src), "n"(sizeof(T)) : "memory");
+}
+// Bounded: after `limit` polls the flag goes up, later waits give up sooner and the kernel runs to its end on what is there.
+__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, uint32_t& limit) {
+    const uint32_t addr = smem_addr(bar);
+    for (uint32_t i = 0; i < limit; ++i) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done)
+                     : "r"(addr), "r"(parity)
+                     : "memory");
+        if (done) return;
+    }
+    limit = POLLS >> 10;
+    atomicExch(&g_ln_timeout, 1);
+}
+
+template <class T>
+constexpr int UNIT = 16 / static_cast<int>(sizeof(T));  // elements of 16 bytes
+
+template <class T>
+__device__ __forceinline__ int misalignment(const T* p) {
+    return static_cast<int>(reinterpret_cast<uintptr_t>(p) / sizeof(T)) & (UNIT<T> - 1);
+}
+
+// How a run of n elements at p splits at 16-byte boundaries: `head` elements, `mid` in whole units, `tail`.  In shared memory
+// element i lies at buf[mis + i], so that the whole units stay aligned.
+template <class T>
+struct Split {
+    int mis, head, mid, tail;
+    __device__ __forceinline__ Split(const T* p, int n) {
+        mis = misalignment(p);
+        head = min((UNIT<T> - mis) % UNIT<T>, n);
+        mid = (n - head) / UNIT<T> * UNIT<T>;
+        tail = n - head - mid;
+    }
+};
+
+// Fetches a run of n elements into `buf` (the first lane of the warp, after its expect_tx) ...
+template <class T>
+__device__ __forceinline__ void fetch_units(T* buf, const T* p, const Split<T>& s, uint64_t* bar) {
+    if (s.mid) bulk_load(buf + s.mis + s.head, p + s.head, static_cast<uint32_t>(s.mid * sizeof(T)), bar);
+}
+// ... and its ends, by eight lanes: k = 0 .. 7.
+template <class T>
+__device__ __forceinline__ void fetch_ends(T* buf, const T* p, int n, int k) {
+    const Split<T> s(p, n);
+    const int i = k < 4 ? k : s.head + s.mid + k - 4;
+    if (k < 4 ? k < s.head : k - 4 < s.tail) copy_one(buf + s.mis + i, p + i);
+}
+
+// Which columns a thread holds.  A row is cut into the 16-byte units of the result's memory: unit u of a row that starts `mis`
+// elements behind a boundary holds columns u UNIT - mis ..., so whole units are stored at once whatever the row's length.
+// Vector j of thread t is unit u0 + j TPR + t.  A group only walks rows of one misalignment, so its columns stay its own.
+template <class T, int TPR, int NV>
+struct Columns {
+    int mis, u0, cols, t;  // cols: where the columns of this CTA end
+    __device__ __forceinline__ int first(int j) const { return (u0 + j * TPR + t) * UNIT<T> - mis; }
+    __device__ __forceinline__ bool some(int j) const { return first(j) < cols; }
+    __device__ __forceinline__ bool whole(int j) const { return first(j) >= 0 && first(j) + UNIT<T> <= cols; }
+    __device__ __forceinline__ bool all_whole() const {
+        bool w = true;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) w &= whole(j);
+        return w;
+    }
+};
+
+struct SpanShape {
+    int64_t rows, pitch_x, pitch_g, pitch_ref;
+    int cols;   // of a row
+    int units;  // 16-byte units of one CTA of the cluster
+    int r;      // rows of a span
+    int spans;
+    int ring;  // slots
+    int cap;   // elements of a slot's buffer
+};
+
+// A unit from shared memory: one 16-byte load, or (where the operand's rows start at another misalignment than the result's)
+// element by element.
+template <class T, bool SAME>
+__device__ __forceinline__ void load_unit(const T* p, Pair<T> (&v)[UNIT<T> / 2]) {
+    if constexpr (SAME) {
+        struct alignas(16) Raw {
+            Pair<T> v[UNIT<T> / 2];
+        };
+        const Raw r = *reinterpret_cast<const Raw*>(p);
+#pragma unroll
+        for (int i = 0; i < UNIT<T> / 2; ++i) v[i] = r.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < UNIT<T> / 2; ++i) v[i] = pair(p[2 * i], p[2 * i + 1]);
+    }
+}
+template <class T>
+__device__ __forceinline__ void store_unit(T* p, const Pair<T> (&v)[UNIT<T> / 2]) {
+    struct alignas(16) Raw {
+        Pair<T> v[UNIT<T> / 2];
+    } r;
+#pragma unroll
+    for (int i = 0; i < UNIT<T> / 2; ++i) r.v[i] = v[i];
+    *reinterpret_cast<Raw*>(p) = r;
+}
+// The elements of a unit at columns c, c + 1, ... that lie in the row.
+template <class T>
+__device__ __forceinline__ void store_part(T* row, int c, int cols, const Pair<T> (&v)[UNIT<T> / 2]) {
+#pragma unroll
+    for (int i = 0; i < UNIT<T> / 2; ++i) {
+        T a, b;
+        unpair(v[i], a, b);
+        if (c + 2 * i >= 0 && c + 2 * i < cols) row[c + 2 * i] = a;
+        if (c + 2 * i + 1 >= 0 && c + 2 * i + 1 < cols) row[c + 2 * i + 1] = b;
+    }
+}
+template <class T>
+__device__ __forceinline__ void replace_outside(int c, int cols, const T& with, Pair<T> (&v)[UNIT<T> / 2]) {
+#pragma unroll
+    for (int i = 0; i < UNIT<T> / 2; ++i) {
+        T a, b;
+        unpair(v[i], a, b);
+        if (c + 2 * i < 0 || c + 2 * i >= cols) a = with;
+        if (c + 2 * i + 1 < 0 || c + 2 * i + 1 >= cols) b = with;
+        v[i] = pair(a, b);
+    }
+}
+
+constexpr int SPAN_THREADS = 512;
+
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Adds the CTAs' sums of a row over the cluster: every CTA's to every CTA; two buffers in turn, as in row_sum.
+template <class T, int CL, int K>
+__device__ __forceinline__ void cluster_sum(T (&s)[K], T (*peers)[CL][2], int rank, unsigned int turn) {
+    T(*to)[2] = peers[turn & 1];
+    if (threadIdx.x < CL) {
+        uint32_t remote;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(to[rank])), "r"(threadIdx.x));
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if constexpr (sizeof(T) == 4) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote + 4 * k), "f"(s[k]) : "memory");
+            else asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote + 8 * k), "d"(s[k]) : "memory");
+        }
+    }
+    cluster_sync();
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] = 0;
+#pragma unroll
+    for (int q = 0; q < CL; ++q)
+#pragma unroll
+        for (int k = 0; k < K; ++k) s[k] += to[q][k];
+}
+
+// Backward.  TPR threads hold a row; narrower rows share a warp.  The weight's and the bias's gradients of a thread's columns
+// stay in its registers over all rows it sees; at the end the threads of a column are joined in shared memory and the block
+// leaves one row of partials.  Rows wider than 512 threads hold are cut over the CTAs of a cluster, which exchange the
+// two sums.
+// How rows lie to 16-byte boundaries.  ALIGNED: every row of x, dy and the result starts and ends on one, so no unit is cut.
+// The others cut units at the rows' ends.  SHIFTED: the three share each row's misalignment and a slot holds one row, between
+// zeros that no copy writes over.  PACKED: they share it, but rows lie end to end in a slot.  MIXED: they do not share it; x
+// and dy are read from shared memory element by element.  In the last two a cut unit's foreign elements are replaced.
+enum { ALIGNED, SHIFTED, PACKED, MIXED };
+template <class T, int TPR, int NV, int CL, int MODE>
+__global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* __restrict__ x, const T* __restrict__ dy,
+                                                                                          const SpanShape sh, const T* __restrict__ w,
+                                                                                          const T* __restrict__ mean, const T* __restrict__ rstd,
+                                                                                          T inv_cols, const T* ref, T* __restrict__ dx,
+                                                                                          T* __restrict__ parts) {
+    constexpr int N = SPAN_THREADS, GT = TPR < 32 ? 32 : TPR, G = N / GT, SUBS = GT / TPR, U = UNIT<T>, H = U / 2, E = NV * U, LINES = N / TPR;
+    constexpr bool HALVES = TPR >= 256;
+    static_assert(CL == 1 || LINES == 1, "a cluster's row takes the whole block");
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    Pack<T, VEC>* ring = reinterpret_cast<Pack<T, VEC>*>(smem_raw);  // [DEPTH][2][NV][THREADS_B]
     __shared__ T part[G][TPR > 32 ? 4 * TPR / 32 : 1];
+    __shared__ T peers[CL > 1 ? 2 : 1][CL][2];
+    __shared__ uint64_t full[G][MOST_RING];
+    __shared__ int line_mis[LINES];
     wb_pdl_enter();
-    const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
-    const int64_t groups = static_cast<int64_t>(gridDim.x) * G, first = static_cast<int64_t>(blockIdx.x) * G + group;
-    auto slot = [&](int stage, int which, int j) -> Pack<T, VEC>& { return ring[((stage * 2 + which) * NV + j) * THREADS_B + threadIdx.x]; };
-    T wv[E], aw[E], ab[E];
+    const int group = threadIdx.x / GT, g = threadIdx.x % GT, sub = g / TPR;
+    const int rank = CL > 1 ? static_cast<int>(blockIdx.x) % CL : 0;
+    const int slab = static_cast<int>(blockIdx.x) / CL, slabs = static_cast<int>(gridDim.x) / CL;
+    const int groups = slabs * G, first = slab * G + group;
+    Columns<T, TPR, NV> col;
+    col.t = g % TPR;
+    col.u0 = rank * sh.units;
+    col.mis = misalignment(ref + (static_cast<int64_t>(first) * sh.r + sub) * sh.pitch_ref);
+    const int from = CL > 1 ? max(0, col.u0 * U - col.mis) : 0;  // this CTA's columns [from, to)
+    const int to = CL > 1 ? min(sh.cols, (col.u0 + sh.units) * U - col.mis) : sh.cols;
+    col.cols = to;
+    const bool whole = col.all_whole();
+    // ring slot: a unit of room, x, a unit of room, dy, mean [32], rstd [32]
+    const int slot_elems = 2 * sh.cap + 64;
+    T* ring = reinterpret_cast<T*>(smem_raw) + group * sh.ring * slot_elems + U;
+    if (g < sh.ring) bar_init(&full[group][g]);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+    if constexpr (CL > 1) cluster_sync();
+    if constexpr (MODE == SHIFTED) {  // the ends of each buffer: a unit before and after the first, all from the last on
+        for (int k = 0; k < 2 * sh.ring && g < 32; ++k) {
+            T* buf = ring + k / 2 * slot_elems + k % 2 * sh.cap;
+            const int e = g < 2 * U ? g - U : max(U, to - from - U) + g - 2 * U;
+            if (e < sh.cap - U) buf[e] = 0;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+    }
+
+    Pair<T> wv[NV][H], aw[NV][H], ab[NV][H];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int c = (j * TPR + t) * VEC + i;
-            wv[j * VEC + i] = c < cols ? (w ? w[c] : T(1)) : T(0);
-            aw[j * VEC + i] = ab[j * VEC + i] = 0;
-            // columns behind the row's end: their slots are never copied to and stay 0
-            for (int d = 0; d < DEPTH; ++d) slot(d, 0, j).v[i] = slot(d, 1, j).v[i] = 0;
+        for (int i = 0; i < H; ++i) {
+            const int c = col.first(j) + 2 * i;
+            const bool a = c >= from && c < to, b = c + 1 >= from && c + 1 < to;
+            wv[j][i] = pair(a ? (w ? w[c] : T(1)) : T(0), b ? (w ? w[c + 1] : T(1)) : T(0));
+            aw[j][i] = ab[j][i] = pair(T(0), T(0));
         }
-    auto fetch = [&](int64_t row, int stage) {
-        if (row < rows) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int c = (j * TPR + t) * VEC;
-                if (c < cols) {
-                    async_copy(&slot(stage, 0, j), x + row * pitch_x + c, std::integral_constant<int, sizeof(T) * VEC>{});
-                    async_copy(&slot(stage, 1, j), dy + row * pitch_g + c, std::integral_constant<int, sizeof(T) * VEC>{});
+
+    // Fetches a span, or the first (x and the small copies) or second (dy) part of it: part 0, 1 or 2.
+    auto fetch = [&](int span, int slot, int part) {
+        if (g >= 32) return;
+        if (span < sh.spans) {
+            const int64_t row0 = static_cast<int64_t>(span) * sh.r;
+            const int nr = static_cast<int>(min(static_cast<int64_t>(sh.r), sh.rows - row0));
+            const int n = sh.r > 1 ? nr * sh.cols : to - from;
+            T* base = ring + slot * slot_elems;
+            const T* px = x + row0 * sh.pitch_x + from;
+            const T* pg = dy + row0 * sh.pitch_g + from;
+            if (g == 0) {
+                const Split<T> sx(px, n), sg(pg, n);
+                if (part != 2) {
+                    bar_expect(&full[group][slot], static_cast<uint32_t>((sx.mid + sg.mid) * sizeof(T)));
+                    fetch_units(base, px, sx, &full[group][slot]);
+                }
+                if (part != 1) fetch_units(base + sh.cap, pg, sg, &full[group][slot]);
+            }
+            if (part != 2) {
+                if (MODE != ALIGNED && g < 16) fetch_ends(base + (g < 8 ? 0 : sh.cap), g < 8 ? px : pg, n, g & 7);
+                if (g < nr) {
+                    copy_one(base + 2 * sh.cap - U + g, mean + row0 + g);
+                    copy_one(base + 2 * sh.cap - U + 32 + g, rstd + row0 + g);
                 }
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (part != 2) asm volatile("cp.async.commit_group;" ::: "memory");
     };
-#pragma unroll
-    for (int d = 0; d < DEPTH - 1; ++d) fetch(first + d * groups, d);
-    T mu = 0, rs = 0;
-    if (first < rows) {
-        mu = mean[first];
-        rs = rstd[first];
-    }
+    // As many spans as the ring has slots are under way at a time.  A slot is filled again as soon as every thread of the
+    // group holds the slot's values in registers: in rows of more than a warp that is at the barrier inside the row's sum.
+    // Before that barrier the small copies of the next span have arrived, so that it makes them known, too.
+    auto settle = [&](int pending) {
+        if (pending <= 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else if (pending == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+        else asm volatile("cp.async.wait_group 3;" ::: "memory");
+    };
+    for (int k = 0; k < sh.ring; ++k) fetch(first + k * groups, k, 0);
+    settle(sh.ring - 1);
+    __syncthreads();
+
     unsigned int turn = 0;
-    int stage = 0;
-    // groups narrower than a warp share its shuffles: they all walk as far as the warp's first one
-    const int64_t lead = TPR < 32 ? first - group % (32 / (TPR < 32 ? TPR : 32)) : first;
-    for (int64_t row = first, at = lead; at < rows; row += groups, at += groups) {
-        fetch(row + (DEPTH - 1) * groups, stage == 0 ? DEPTH - 1 : stage - 1);
-        T mu_next = 0, rs_next = 0;
-        if (row + groups < rows) {
-            mu_next = mean[row + groups];
-            rs_next = rstd[row + groups];
+    uint32_t limit = POLLS, phase = 0;
+    int slot = 0;
+    for (int span = first; span < sh.spans; span += groups) {
+        bar_wait(&full[group][slot], phase, limit);
+        if (HALVES && span != first) fetch(span + (sh.ring - 1) * groups, slot == 0 ? sh.ring - 1 : slot - 1, 2);
+        const int64_t row0 = static_cast<int64_t>(span) * sh.r;
+        const int nr = static_cast<int>(min(static_cast<int64_t>(sh.r), sh.rows - row0));
+        const T* base = ring + slot * slot_elems;
+        // unit j of row r starts at base[off + r cols + (j TPR + t) U]
+        const int shift = col.u0 * U - col.mis - from + col.t * U;
+        const T *span_x = base + shift, *span_g = base + sh.cap + shift;
+        if (MODE != ALIGNED) {
+            span_x += misalignment(x + row0 * sh.pitch_x + from);
+            span_g += misalignment(dy + row0 * sh.pitch_g + from);
         }
-        asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
-        const bool live = TPR >= 32 || row < rows;
-        T xh[E], g[E], s[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const Pack<T, VEC> px = slot(stage, 0, j), pg = slot(stage, 1, j);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int e = j * VEC + i;
-                const T up = live ? pg.v[i] : T(0);
-                xh[e] = live ? (px.v[i] - mu) * rs : T(0);  // not live: the slot holds an older row
-                aw[e] += up * xh[e];
-                ab[e] += up;
-                g[e] = up * wv[e];
-                s[0] += g[e];
-                s[1] += g[e] * xh[e];
-            }
-        }
-        if (dx) {
-            row_sum<T, TPR, 2>(s, part[group], 1 + group, turn);
-            const T c0 = s[0] * inv_cols, c1 = s[1] * inv_cols;
-            if (live) {
-                T* dr = dx + row * cols;
+        for (int r0 = 0; r0 < nr; r0 += SUBS) {  // the same number of turns for every lane of a warp
+            const bool live = SUBS == 1 || r0 + sub < nr;
+            const int r = live ? r0 + sub : r0;
+            const T *bx = span_x + r * sh.cols, *bg = span_g + r * sh.cols;
+            const T mu = base[2 * sh.cap - U + r], rs = base[2 * sh.cap - U + 32 + r];
+            const Pair<T> minus_mu = pair(-mu, -mu), rs2 = pair(rs, rs);
+            Pair<T> xh[NV][H], gv[NV][H], s0 = pair(T(0), T(0)), s1 = s0;
+            auto take = [&](auto edges) {
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
-                    const int c = (j * TPR + t) * VEC;
-                    Pack<T, VEC> o;
+                    // a unit behind the row's end (of the last vector only, in a row of its own): any that is there
+                    const int at = (CL == 1 && j < NV - 1) || col.some(j) ? j * TPR * U : -col.t * U;
+                    Pair<T> up[H];
+                    load_unit<T, MODE != MIXED>(bx + at, xh[j]);
+                    load_unit<T, MODE != MIXED>(bg + at, up);
+                    if constexpr (decltype(edges)::value) {  // what is not of this row counts as a mean value without gradient
+                        replace_outside(col.first(j), to, mu, xh[j]);
+                        replace_outside(col.first(j), to, T(0), up);
+                    }
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) o.v[i] = rs * (g[j * VEC + i] - c0 - xh[j * VEC + i] * c1);
-                    if (c < cols) *reinterpret_cast<Pack<T, VEC>*>(dr + c) = o;
+                    for (int i = 0; i < H; ++i) {
+                        xh[j][i] = (xh[j][i] + minus_mu) * rs2;
+                        gv[j][i] = up[i] * wv[j][i];
+                        aw[j][i] = muladd(up[i], xh[j][i], aw[j][i]);
+                        ab[j][i] = ab[j][i] + up[i];
+                        s0 = s0 + gv[j][i];
+                        s1 = muladd(gv[j][i], xh[j][i], s1);
+                    }
+                }
+            };
+            if (live) {
+                if (MODE == ALIGNED || MODE == SHIFTED || whole) take(std::false_type{});
+                else take(std::true_type{});
+            }
+            if (!dx) continue;
+            T s[2], lo, hi;
+            unpair(s0, lo, hi);
+            s[0] = lo + hi;
+            unpair(s1, lo, hi);
+            s[1] = lo + hi;
+            if constexpr (TPR > 32) settle(sh.ring - 2);
+            row_sum<T, TPR, G, 2>(s, part[group], 1 + group, turn, [&]() { fetch(span + sh.ring * groups, slot, HALVES ? 1 : 0); });
+            if constexpr (CL > 1) cluster_sum<T, CL, 2>(s, peers, rank, turn);
+            const T k0 = -rs * (s[0] * inv_cols), k1 = -rs * (s[1] * inv_cols);
+            const Pair<T> k0p = pair(k0, k0), k1p = pair(k1, k1);
+            if (live) {
+                T* dr = dx + (row0 + r) * sh.cols;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    Pair<T> o[H];
+#pragma unroll
+                    for (int i = 0; i < H; ++i) o[i] = muladd(gv[j][i], rs2, muladd(xh[j][i], k1p, k0p));
+                    if (MODE == ALIGNED ? (CL == 1 && j < NV - 1) || col.some(j) : whole || col.whole(j)) store_unit(dr + col.first(j), o);
+                    else if (MODE != ALIGNED) store_part(dr, col.first(j), to, o);
                 }
             }
         }
-        mu = mu_next;
-        rs = rs_next;
-        stage = stage + 1 == DEPTH ? 0 : stage + 1;
+        if (GT == 32 || !dx) {
+            settle(sh.ring - 2);
+            if constexpr (GT == 32) __syncwarp();
+            else if constexpr (G == 1) __syncthreads();
+            else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(GT) : "memory");
+            fetch(span + sh.ring * groups, slot, HALVES ? 1 : 0);
+        }
+        slot = slot == sh.ring - 1 ? 0 : slot + 1;
+        phase ^= slot == 0;
     }
     if (!parts) return;
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    if constexpr (G > 1) {  // the groups' sums, in the groups' order
-        T* joined = reinterpret_cast<T*>(smem_raw);  // [2][G][TPR E]
-        __syncthreads();
+    __syncthreads();
+    // one line for each row that the block holds at a time, added up in order
+    T* joined = reinterpret_cast<T*>(smem_raw);  // [2][LINES][TPR E]
+    const int line = threadIdx.x / TPR;
+    if (col.t == 0) line_mis[line] = col.mis;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int c = (j * TPR + t) * VEC + i;
-                joined[group * TPR * E + c] = aw[j * VEC + i];
-                joined[(G + group) * TPR * E + c] = ab[j * VEC + i];
-            }
-        __syncthreads();
-        for (int c = threadIdx.x; c < cols; c += THREADS_B) {
-            T sw = joined[c], sb = joined[G * TPR * E + c];
-            for (int k = 1; k < G; ++k) {
-                sw += joined[k * TPR * E + c];
-                sb += joined[(G + k) * TPR * E + c];
-            }
-            parts[static_cast<int64_t>(blockIdx.x) * cols + c] = sw;
-            parts[static_cast<int64_t>(gridDim.x + blockIdx.x) * cols + c] = sb;
+    for (int j = 0; j < NV; ++j) {
+        T* a = joined + line * TPR * E + (j * TPR + col.t) * U;
+        store_unit(a, aw[j]);
+        store_unit(a + LINES * TPR * E, ab[j]);
+    }
+    __syncthreads();
+    for (int c = from + static_cast<int>(threadIdx.x); c < to; c += N) {
+        T sw = 0, sb = 0;
+        for (int k = 0; k < LINES; ++k) {
+            const T* a = joined + k * TPR * E + c + line_mis[k] - col.u0 * U;
+            sw += a[0];
+            sb += a[LINES * TPR * E];
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int c = (j * TPR + t) * VEC + i;
-                if (c < cols) {
-                    parts[static_cast<int64_t>(blockIdx.x) * cols + c] = aw[j * VEC + i];
-                    parts[static_cast<int64_t>(gridDim.x + blockIdx.x) * cols + c] = ab[j * VEC + i];
-                }
-            }
+        parts[static_cast<int64_t>(slab) * sh.cols + c] = sw;
+        parts[static_cast<int64_t>(slabs + slab) * sh.cols + c] = sb;
     }
 }
 
@@ -393,28 +687,42 @@ __global__ void __launch_bounds__(THREADS) ln_dw_any_kernel(const T* __restrict_
     }
 }
 
-// Sums the slabs of both partial arrays: 32 columns per block, eight runs of slabs side by side, joined in order.
+// Sums the slabs of both partial arrays: 32 columns per block, 32 lines of threads that take every 32nd slab, joined in
+// order.  A line's loads (ten for 296 slabs) are all in flight at once: with eight lines and their loads in turn this
+// kernel took 10 us whatever the size.
+constexpr int JOIN_LINES = 32;
 template <class T>
-__global__ void __launch_bounds__(THREADS) ln_dw_join_kernel(const T* __restrict__ parts, int slabs, int64_t cols, T* __restrict__ dw,
-                                                             T* __restrict__ db) {
-    __shared__ double sum[THREADS / 32][32];
+__global__ void __launch_bounds__(32 * JOIN_LINES) ln_dw_join_kernel(const T* __restrict__ parts, int slabs, int64_t cols, T* __restrict__ dw,
+                                                                     T* __restrict__ db) {
+    __shared__ double sum[JOIN_LINES][33];
     wb_pdl_enter();
     T* out = blockIdx.y == 0 ? dw : db;
     if (!out) return;
     const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-    const T* p = parts + static_cast<int64_t>(blockIdx.y) * slabs * cols;
     double acc = 0.0;
     if (c < cols) {
-#pragma unroll 8
-        for (int k = line; k < slabs; k += THREADS / 32) acc += p[static_cast<int64_t>(k) * cols + c];
+        const T* p = parts + static_cast<int64_t>(blockIdx.y) * slabs * cols + c;
+        constexpr int BATCH = 10;
+        for (int k0 = line; k0 < slabs; k0 += JOIN_LINES * BATCH) {
+            T v[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                const int k = k0 + j * JOIN_LINES;
+                v[j] = k < slabs ? p[static_cast<int64_t>(k) * cols] : T(0);
+            }
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) acc += v[j];
+        }
     }
     sum[line][lane] = acc;
     __syncthreads();
-    if (line == 0 && c < cols) {
-        for (int k = 1; k < THREADS / 32; ++k) acc += sum[k][lane];
-        out[c] = static_cast<T>(acc);
-    }
+    // transposed: a warp joins one column
+    acc = sum[lane][line];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
+    const int64_t to = static_cast<int64_t>(blockIdx.x) * 32 + line;
+    if (lane == 0 && to < cols) out[to] = static_cast<T>(acc);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
@@ -503,8 +811,9 @@ struct SpanList {
     }
 };
 
-// Rows are summed in at most this many slabs for the weight's gradient.
-int dw_slabs(int sm_count, int64_t rows) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 2 * sm_count))); }
+// Rows are summed in at most this many slabs for the weight's gradient (a multiple of four groups of them, see
+// launch_spans).
+int dw_slabs(int sm_count, int64_t rows) { return static_cast<int>(std::max<int64_t>(4, std::min<int64_t>((rows + 3) / 4 * 4, 2 * sm_count))); }
 
 // Unit stride along the row and one stride from row to row.
 bool plain_rows(const RowView& v, const Shape& s) { return v.nd_row == 1 && v.nd_col == 1 && (v.st_col[0] == 1 || s.cols == 1); }
@@ -519,21 +828,23 @@ bool rows_aligned(const void* p, int64_t pitch, int64_t cols) {
 
 // Calls f with (threads per row, vectors per thread) for rows of `packs` vectors, at most MOST vectors per thread: the
 // fewest threads that hold the row, so that small rows share a block and the reductions stay short.
-template <int MOST, class F>
+template <int MOST, int LEAST, class F>
 bool choose_row(int64_t packs, F&& f) {
     auto per = [&](auto tpr) -> bool {
         constexpr int TPR = decltype(tpr)::value;
         if (packs > static_cast<int64_t>(TPR) * MOST) return false;
         const int64_t nv = (packs + TPR - 1) / TPR;
-        if constexpr (TPR == 8) {
+        if constexpr (TPR < LEAST) return false;
+        if constexpr (TPR == LEAST) {
             if (nv <= 1) return f(tpr, std::integral_constant<int, 1>{}), true;
             if (nv <= 2) return f(tpr, std::integral_constant<int, 2>{}), true;
+            if constexpr (MOST / 4 > 2)
+                if (nv <= MOST / 4) return f(tpr, std::integral_constant<int, MOST / 4>{}), true;
+            if constexpr (MOST / 2 > 2)
+                if (nv <= MOST / 2) return f(tpr, std::integral_constant<int, MOST / 2>{}), true;
         }
-        if constexpr (TPR == 8 && MOST > 4)
-            if (nv <= MOST / 4) return f(tpr, std::integral_constant<int, MOST / 4>{}), true;
-        if constexpr (TPR == 8)
-            if (nv <= MOST / 2) return f(tpr, std::integral_constant<int, MOST / 2>{}), true;
-        if (nv <= MOST * 3 / 4) return f(tpr, std::integral_constant<int, MOST * 3 / 4>{}), true;
+        if constexpr (MOST >= 4)
+            if (nv <= MOST * 3 / 4) return f(tpr, std::integral_constant<int, MOST * 3 / 4>{}), true;
         return f(tpr, std::integral_constant<int, MOST>{}), true;
     };
     return per(std::integral_constant<int, 8>{}) || per(std::integral_constant<int, 16>{}) || per(std::integral_constant<int, 32>{}) ||
@@ -546,7 +857,7 @@ constexpr int row_elems = 64 / static_cast<int>(sizeof(T));  // elements of a ro
 
 template <class T, int VEC>
 bool fwd_rows(WbBackend* b, const T* x, int64_t pitch, const Shape& s, const T* w, const T* bias, double eps, T* y, T* mean, T* rstd, cudaError_t* err) {
-    return choose_row<row_elems<T> / VEC>((s.cols + VEC - 1) / VEC, [&](auto tpr, auto nv) {
+    return choose_row<row_elems<T> / VEC, 8>((s.cols + VEC - 1) / VEC, [&](auto tpr, auto nv) {
         constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, G = fwd_threads<TPR> / TPR;
         const int64_t grid = (s.rows + G - 1) / G;
         if (grid > INT32_MAX) {
@@ -582,19 +893,152 @@ int fwd_typed(WbBackend* b, const WbView* x, int nd, const Shape& s, const T* w,
     return WB_OK;
 }
 
-template <class T, int VEC>
-bool bwd_rows(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t pitch_g, const Shape& s, const T* w, const T* mean, const T* rstd, T* dx,
-              T* parts, int* slabs, cudaError_t* err) {
-    return choose_row<row_elems<T> / VEC>((s.cols + VEC - 1) / VEC, [&](auto tpr, auto nv) {
-        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, N = bwd_threads<TPR>, G = N / TPR, DEPTH = TPR > 512 ? 1 : 2;
-        constexpr size_t smem = sizeof(T) * 2 * DEPTH * NV * VEC * N;
-        static_assert(smem <= 200 * 1024, "ring");
-        auto kernel = ln_bwd_rows_kernel<T, VEC, TPR, NV, DEPTH>;
-        *err = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (*err != cudaSuccess) return;
-        *slabs = static_cast<int>(std::min<int64_t>(dw_slabs(b->sm_count, s.rows), (s.rows + G - 1) / G));
-        *err = wb_launch_pdl(kernel, dim3(*slabs), dim3(N), smem, b->stream, x, pitch_x, dy, pitch_g, s.rows, static_cast<int>(s.cols), w, mean, rstd,
-                             static_cast<T>(1.0 / static_cast<double>(s.cols)), dx, parts);
+// Rows repeat their misalignment after this many (1, 2 or 4): UNIT / gcd(UNIT, pitch).
+template <class T>
+int period(int64_t pitch) {
+    int p = UNIT<T>;
+    while (p > 1 && pitch % 2 == 0) {
+        p /= 2;
+        pitch /= 2;
+    }
+    return p;
+}
+template <class T>
+bool same_misalignment(const T* a, int64_t pitch_a, const T* b, int64_t pitch_b, int64_t rows) {
+    return (reinterpret_cast<uintptr_t>(a) - reinterpret_cast<uintptr_t>(b)) % 16 == 0 && (rows == 1 || (pitch_a - pitch_b) % UNIT<T> == 0);
+}
+
+cudaLaunchAttribute cluster_attribute(unsigned n) {
+    cudaLaunchAttribute a{};
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = n;
+    a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    return a;
+}
+
+// The grid of a span kernel: as many groups as the device holds at a time or as there are spans, and a multiple of the
+// period, so that a group's rows are all of one misalignment.  Then the launch, as the programmatic dependent of what is
+// before it.
+template <int CL, class... Params, class... Args>
+cudaError_t launch_spans(WbBackend* b, void (*kernel)(Params...), const SpanShape& sh, int threads, int groups, int per_sm, size_t smem, int period,
+                         int* slabs, Args... args) {
+    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(CL);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = b->stream;
+    cudaLaunchAttribute attr[2];
+    unsigned n = 0;
+    int64_t most = b->sm_count * per_sm;
+    if (CL > 1) {
+        // Clusters that are resident at a time: not every processor group is a multiple of CL processors, and a cluster more than
+        // fit runs as a second wave ([4096, 16384] over clusters of 4: 461 us with 37 of them, 267 us with those that fit).
+        int fit = 0;
+        attr[n++] = cluster_attribute(CL);
+        cfg.attrs = attr;
+        cfg.numAttrs = n;
+        e = cudaOccupancyMaxActiveClusters(&fit, reinterpret_cast<const void*>(kernel), &cfg);
+        if (e != cudaSuccess) return e;
+        most = std::min<int64_t>(std::max(fit, 1), most);
+    }
+    const int step = std::max(1, period / groups);
+    int64_t want = std::min<int64_t>(most, (static_cast<int64_t>(sh.spans) + groups - 1) / groups);
+    want = std::min((want + step - 1) / step * step, most / step * step);
+    *slabs = static_cast<int>(std::max<int64_t>(want, step));
+    cfg.gridDim = dim3(static_cast<unsigned>(*slabs * CL));
+    if (wb_pdl_allowed()) {
+        attr[n] = cudaLaunchAttribute{};
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Rows per span: 32 KB per operand and turn of the block, but no more rows than leave every group a span.
+template <class T>
+int rows_per_span(const WbBackend* b, const Shape& s, int groups, int subs) {
+    const int64_t room = 32768 / static_cast<int64_t>(sizeof(T)) / groups / s.cols, all = static_cast<int64_t>(b->sm_count) * groups, share = (s.rows + all - 1) / all;
+    const int64_t r = std::min<int64_t>(std::min<int64_t>(room, share), 32);
+    return static_cast<int>(std::max<int64_t>((r + subs - 1) / subs * subs, 1));
+}
+
+// Slots of the ring, `slots` bytes each for the whole block.  About 128 KB under way on a processor saturate the memory; with
+// more of them some processors' copies wait for others', and since rows are dealt out beforehand the last one decides
+// ([16384, 4096]: 123 us with 2 slots of 64 KB, 149 us with 3).  A cluster's exchange takes longer than that covers.
+int ring_depth(size_t slots, int cl) {
+    const int fit = static_cast<int>((216 << 10) / slots);
+    return std::max(2, std::min({fit, MOST_RING, cl > 1 ? 3 : static_cast<int>(((128 << 10) + slots / 2) / slots)}));
+}
+
+// Threads per row, units per thread and CTAs per row for rows of up to `units` units: the fewest threads that hold the row.
+// Rows that share a warp have to lie end to end (`dense`), and as many of them side by side as the misalignment's period.
+template <class F>
+bool choose_span(int64_t units, bool dense, int period, F&& f) {
+    constexpr int MOST = 4;
+    auto per = [&](auto tpr) -> bool {
+        constexpr int TPR = decltype(tpr)::value;
+        if (units > TPR * MOST || (TPR < 32 && (!dense || 32 / TPR % period != 0))) return false;
+        const int nv = static_cast<int>((units + TPR - 1) / TPR);
+        using One = std::integral_constant<int, 1>;
+        if constexpr (TPR == 8 || TPR == 32) {
+            if (nv <= 1) return f(tpr, One{}, One{}), true;
+            if (nv <= 2) return f(tpr, std::integral_constant<int, 2>{}, One{}), true;
+        }
+        if (nv <= 3) return f(tpr, std::integral_constant<int, 3>{}, One{}), true;
+        return f(tpr, std::integral_constant<int, 4>{}, One{}), true;
+    };
+    if (per(std::integral_constant<int, 8>{}) || per(std::integral_constant<int, 16>{}) || per(std::integral_constant<int, 32>{}) ||
+        per(std::integral_constant<int, 64>{}) || per(std::integral_constant<int, 128>{}) || per(std::integral_constant<int, 256>{}) ||
+        per(std::integral_constant<int, 512>{}))
+        return true;
+    using W = std::integral_constant<int, 512>;
+    using A = std::integral_constant<int, MOST>;
+    if (units <= 2 * 512 * MOST) return f(W{}, A{}, std::integral_constant<int, 2>{}), true;
+    if (units <= 4 * 512 * MOST) return f(W{}, A{}, std::integral_constant<int, 4>{}), true;
+    if (units <= 8 * 512 * MOST) return f(W{}, A{}, std::integral_constant<int, 8>{}), true;
+    return false;
+}
+
+template <class T>
+bool bwd_spans(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t pitch_g, const Shape& s, const T* w, const T* mean, const T* rstd, T* dx,
+               T* parts, int* slabs, cudaError_t* err) {
+    const T* ref = dx ? dx : dy;
+    const int64_t pitch_ref = s.rows == 1 ? 0 : dx ? s.cols : pitch_g;
+    const bool same = same_misalignment<T>(x, pitch_x, ref, pitch_ref, s.rows) && same_misalignment<T>(dy, pitch_g, ref, pitch_ref, s.rows);
+    const bool dense = pitch_x == s.cols && pitch_g == s.cols;
+    const int per = period<T>(pitch_ref);
+    const bool aligned = per == 1 && reinterpret_cast<uintptr_t>(ref) % 16 == 0;
+    const int64_t units = (s.cols + UNIT<T> - 1 + (aligned ? 0 : UNIT<T> - 1)) / UNIT<T>;
+    return choose_span(units, dense, per, [&](auto tpr, auto nv, auto cl) {
+        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, CL = decltype(cl)::value;
+        constexpr int N = SPAN_THREADS, GT = TPR < 32 ? 32 : TPR, G = N / GT, SUBS = GT / TPR;
+        SpanShape sh;
+        sh.rows = s.rows;
+        sh.cols = static_cast<int>(s.cols);
+        sh.pitch_x = pitch_x;
+        sh.pitch_g = pitch_g;
+        sh.pitch_ref = pitch_ref;
+        sh.units = static_cast<int>((units + CL - 1) / CL);
+        const bool cut = !aligned || s.cols % UNIT<T> != 0;
+        sh.r = GT == 32 && dense && SUBS % per == 0 && (SUBS > 1 || !cut) ? rows_per_span<T>(b, s, G, SUBS) : 1;
+        sh.spans = static_cast<int>((s.rows + sh.r - 1) / sh.r);
+        // behind a unit of room: the misalignment, the rows, what a last unit reads behind them
+        const int64_t run = CL > 1 ? static_cast<int64_t>(sh.units) * UNIT<T> : sh.r * s.cols;
+        sh.cap = static_cast<int>((run + UNIT<T> - 1) / UNIT<T> * UNIT<T> + 3 * UNIT<T>);
+        const size_t slots = sizeof(T) * static_cast<size_t>(G) * (2 * sh.cap + 64), join = sizeof(T) * 2 * N * NV * UNIT<T>;
+        sh.ring = ring_depth(slots, CL);
+        auto go = [&](auto kernel) {
+            *err = launch_spans<CL>(b, kernel, sh, N, G, 1, std::max(slots * sh.ring, join), sh.r > 1 ? 1 : per, slabs, x, dy, sh, w, mean, rstd,
+                                    static_cast<T>(1.0 / static_cast<double>(s.cols)), ref, dx, parts);
+        };
+        if (!same) go(ln_bwd_span_kernel<T, TPR, NV, CL, MIXED>);
+        else if (!cut) go(ln_bwd_span_kernel<T, TPR, NV, CL, ALIGNED>);
+        else if constexpr (SUBS > 1) go(ln_bwd_span_kernel<T, TPR, NV, CL, PACKED>);
+        else go(ln_bwd_span_kernel<T, TPR, NV, CL, SHIFTED>);
     });
 }
 
@@ -609,13 +1053,8 @@ int bwd_typed(WbBackend* b, const WbView* x, const WbView* dy, int nd, const Sha
     cudaError_t err = cudaSuccess;
     bool done = false;
     int slabs = dw_slabs(b->sm_count, s.rows);
-    if (plain_rows(vx, s) && plain_rows(vg, s)) {
-        const int64_t px = vx.st_row[0], pg = vg.st_row[0];
-        T* to = sums ? parts : nullptr;
-        if (rows_aligned<T>(xp, px, s.cols) && rows_aligned<T>(gp, pg, s.cols) && rows_aligned<T>(dx, s.cols, s.cols))
-            done = bwd_rows<T, wide<T>>(b, xp, px, gp, pg, s, w, mean, rstd, dx, to, &slabs, &err);
-        else
-            done = bwd_rows<T, 1>(b, xp, px, gp, pg, s, w, mean, rstd, dx, to, &slabs, &err);
+    if (plain_rows(vx, s) && plain_rows(vg, s) && s.rows < (1 << 30)) {
+        done = bwd_spans<T>(b, xp, vx.st_row[0], gp, vg.st_row[0], s, w, mean, rstd, dx, sums ? parts : nullptr, &slabs, &err);
         if (done) {
             WB_CHECK_CUDA(err);
             WB_LAUNCH_OK(b);
@@ -633,7 +1072,7 @@ int bwd_typed(WbBackend* b, const WbView* x, const WbView* dy, int nd, const Sha
                                     parts, slabs));
         WB_LAUNCH_OK(b);
     }
-    WB_CHECK_CUDA(wb_launch_pdl(ln_dw_join_kernel<T>, dim3(static_cast<unsigned>((s.cols + 31) / 32), 2), dim3(THREADS), 0, b->stream,
+    WB_CHECK_CUDA(wb_launch_pdl(ln_dw_join_kernel<T>, dim3(static_cast<unsigned>((s.cols + 31) / 32), 2), dim3(32 * JOIN_LINES), 0, b->stream,
                                 static_cast<const T*>(parts), slabs, s.cols, dw, db));
     WB_LAUNCH_OK(b);
     return WB_OK;
@@ -645,6 +1084,21 @@ int64_t bwd_workspace(int sm_count, int64_t rows, int64_t cols, int dtype) {
 }
 
 }  // namespace
+
+// Reads and clears the flag of the bounded waits above; waits for the stream.
+int wb_layer_norm_check(WbBackend* b) {
+    WbDeviceGuard dev(b->ordinal);
+    WB_CHECK_CUDA(dev.status);
+    int raised = 0;
+    WB_CHECK_CUDA(cudaMemcpyFromSymbolAsync(&raised, g_ln_timeout, sizeof(int), 0, cudaMemcpyDeviceToHost, b->stream));
+    WB_CHECK_CUDA(cudaStreamSynchronize(b->stream));
+    if (!raised) return WB_OK;
+    const int zero = 0;
+    WB_CHECK_CUDA(cudaMemcpyToSymbolAsync(g_ln_timeout, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, b->stream));
+    WB_CHECK_CUDA(cudaStreamSynchronize(b->stream));
+    wb_set_error("a layer norm gave up waiting for a bulk copy");
+    return WB_ERR_TIMEOUT;
+}
 
 // ---- entry points ------------------------------------------------------------------------------------------
 
