@@ -17,6 +17,7 @@
 
 #include "adam.cuh"
 #include "common.h"
+#include "pair.cuh"
 
 namespace {
 
@@ -66,31 +67,77 @@ __device__ __forceinline__ AdamK with_device_scale(AdamK k, const float* scale) 
 
 // ---- 32-bit state -------------------------------------------------------------------------------------------
 
+__device__ __forceinline__ void one(float* th, const float* g, float* m, float* v, int i, const AdamK& k) {
+    float a = th[i], mi = k.first ? 0.f : m[i], vi = k.first ? 0.f : v[i];
+    adam_one(a, g[i], mi, vi, k);
+    th[i] = a;
+    m[i] = mi;
+    v[i] = vi;
+}
+
+// A tensor whose pointers are both on 16-byte boundaries takes 128-bit accesses (the state always is); any other, and a
+// tensor's last group, goes element by element.
 template <int N>
 __global__ void __launch_bounds__(THREADS) adam_multi32_kernel(const __grid_constant__ Table<N> tab, float* __restrict__ m, float* __restrict__ v,
                                                                AdamK k0, const float* __restrict__ scale) {
     wb_pdl_enter();
-    const AdamK k = with_device_scale(k0, scale);
     const int ti = find_tensor(tab, blockIdx.x);
     const Tensor t = tab.t[ti];
     if (!t.grad) return;
-    const int64_t len = t.len < 0 ? -t.len : t.len;
-    AdamK kt = k;
-    if (t.len < 0) kt.has_wd = 0;
-    const int64_t at = static_cast<int64_t>(blockIdx.x - tab.first[ti]) * CHUNK, end = min(at + CHUNK, len);
-    for (int64_t i = at + threadIdx.x; i < end; i += THREADS) {
-        float th = t.theta[i], mi = k.first ? 0.f : m[t.offset + i], vi = k.first ? 0.f : v[t.offset + i];
-        adam_one(th, t.grad[i], mi, vi, kt);
-        t.theta[i] = th;
-        m[t.offset + i] = mi;
-        v[t.offset + i] = vi;
+    AdamK k = with_device_scale(k0, scale);
+    const int64_t len = t.len < 0 ? -t.len : t.len, at = static_cast<int64_t>(blockIdx.x - tab.first[ti]) * CHUNK;
+    if (t.len < 0) k.has_wd = 0;
+    float *th = t.theta + at, *mp = m + t.offset + at, *vp = v + t.offset + at;
+    const float* gp = t.grad + at;
+    const int n = static_cast<int>(min(CHUNK, len - at));
+    if (((reinterpret_cast<uintptr_t>(t.theta) | reinterpret_cast<uintptr_t>(t.grad)) & 15) == 0) {
+        constexpr int U = static_cast<int>(CHUNK) / (4 * THREADS);
+        float4 a[U], g[U], mi[U], vi[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (u * THREADS + threadIdx.x) * 4;
+            if (i + 4 <= n) {
+                a[u] = *reinterpret_cast<const float4*>(th + i);
+                g[u] = *reinterpret_cast<const float4*>(gp + i);
+                mi[u] = k.first ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(mp + i);
+                vi[u] = k.first ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(vp + i);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (u * THREADS + threadIdx.x) * 4;
+            if (i + 4 <= n) {
+                adam_one(a[u].x, g[u].x, mi[u].x, vi[u].x, k);
+                adam_one(a[u].y, g[u].y, mi[u].y, vi[u].y, k);
+                adam_one(a[u].z, g[u].z, mi[u].z, vi[u].z, k);
+                adam_one(a[u].w, g[u].w, mi[u].w, vi[u].w, k);
+                *reinterpret_cast<float4*>(th + i) = a[u];
+                *reinterpret_cast<float4*>(mp + i) = mi[u];
+                *reinterpret_cast<float4*>(vp + i) = vi[u];
+            }
+        }
+        const int i = (n & ~3) + static_cast<int>(threadIdx.x);
+        if (i < n) one(th, gp, mp, vp, i, k);
+    } else {
+        for (int i = threadIdx.x; i < n; i += THREADS) one(th, gp, mp, vp, i, k);
     }
 }
 
 // ---- 8-bit state --------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ float decode_m(int c, float unit) { return static_cast<float>(c * abs(c)) * unit; }
-__device__ __forceinline__ float decode_root(int c, float unit) { return static_cast<float>(c * c) * unit; }
+// A byte as f32 without the conversion unit (16 lanes per clock, which the square roots and the division need): put under
+// the exponent of 2^23 it is 2^23 + byte, exactly; and a value in [0, 255] plus 2^23 is rounded to the nearest integer, ties
+// to even, which then is the low byte.
+constexpr float MAGIC = 8388608.f;
+__device__ __forceinline__ float byte_of(uint32_t word, int i, float minus) { return __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7440 + i)) + minus; }
+__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// c |c| unit and (c c unit)^2 for the values c of the codes.
+__device__ __forceinline__ float decode_m(float c, float unit) { return c * fabsf(c) * unit; }
+__device__ __forceinline__ float decode_root(float c, float unit) { return c * c * unit; }
+__device__ __forceinline__ float m_code(uint32_t word, int i) { return byte_of(word ^ 0x80808080u, i, -(MAGIC + 128.f)); }
+__device__ __forceinline__ float v_code(uint32_t word, int i) { return byte_of(word, i, -MAGIC); }
 
 // The scale of a block whose largest magnitude has these bits.  One that is not finite poisons the block: its scale is
 // stored as NaN, and every value read from it is NaN.
@@ -98,83 +145,182 @@ __device__ __forceinline__ float block_scale(unsigned int bits) {
     if (bits >= 0x7f800000u) return __int_as_float(0x7fffffff);
     return fmaxf(__uint_as_float(bits), TINY);
 }
-__device__ __forceinline__ int encode(float magnitude, float level, float top) {
-    return __float2int_rn(fminf(sqrtf(magnitude * level), top));
+
+// Codes of eight magnitudes: min(rint(sqrt(x level)), top), the square root correctly rounded.  The approximate one is off by
+// less than 2^-20 of at most 256, which moves rint's result only next to a half: a lane that comes within 2^-11 of one
+// takes all its roots again.  Each result is 2^23 + code.
+__device__ __forceinline__ void encode(const float (&x)[8], float level, float top, uint32_t (&code)[8]) {
+    float far = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float s;
+        asm("sqrt.approx.f32 %0, %1;" : "=f"(s) : "f"(x[j] * level));
+        s = fminf(s, top);
+        const float r = s + MAGIC;
+        far = fmaxf(far, fabsf(s - (r - MAGIC)));
+        code[j] = __float_as_uint(r);
+    }
+    if (far > 0.49951171875f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) code[j] = __float_as_uint(fminf(sqrtf(x[j] * level), top) + MAGIC);
+    }
 }
 
+// One warp takes a block of 256 elements, a lane the groups of four at 4 lane and 128 + 4 lane.
 template <int N>
-__global__ void __launch_bounds__(THREADS) adam_multi8_kernel(const __grid_constant__ Table<N> tab, int8_t* __restrict__ mc, uint8_t* __restrict__ vc,
+__global__ void __launch_bounds__(THREADS) adam_multi8_kernel(const __grid_constant__ Table<N> tab, uint32_t* __restrict__ mc, uint32_t* __restrict__ vc,
                                                               float* __restrict__ ms, float* __restrict__ vs, AdamK k0,
-                                                              const float* __restrict__ scale) {
+                                                              const float* __restrict__ scale, float minus_zero) {
     wb_pdl_enter();
-    const AdamK k = with_device_scale(k0, scale);
     const int ti = find_tensor(tab, blockIdx.x);
     const Tensor t = tab.t[ti];
     if (!t.grad) return;
     const int64_t len = t.len < 0 ? -t.len : t.len;
-    AdamK kt = k;
-    if (t.len < 0) kt.has_wd = 0;
-    const int lane = threadIdx.x & 31;
     const int64_t at = static_cast<int64_t>(blockIdx.x - tab.first[ti]) * CHUNK + (threadIdx.x >> 5) * BLOCK8;
     if (at >= len) return;
+    AdamK k = with_device_scale(k0, scale);
+    if (t.len < 0) k.has_wd = 0;
+    const int lane = threadIdx.x & 31, n = static_cast<int>(min(static_cast<int64_t>(BLOCK8), len - at));
     const int64_t s = t.offset + at, block = s / BLOCK8;
-    const float um = k.first ? 0.f : ms[block] * (1.f / (M_TOP * M_TOP)), ur = k.first ? 0.f : vs[block] * (1.f / (V_TOP * V_TOP));
+    float* tp = t.theta + at;
+    const float* gp = t.grad + at;
+    float th[8], g[8];
+    const bool wide = n == BLOCK8 && ((reinterpret_cast<uintptr_t>(t.theta) | reinterpret_cast<uintptr_t>(t.grad)) & 15) == 0;
+    if (wide) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float4 a = *reinterpret_cast<const float4*>(tp + h * 128 + lane * 4), b = *reinterpret_cast<const float4*>(gp + h * 128 + lane * 4);
+            th[4 * h] = a.x; th[4 * h + 1] = a.y; th[4 * h + 2] = a.z; th[4 * h + 3] = a.w;
+            g[4 * h] = b.x; g[4 * h + 1] = b.y; g[4 * h + 2] = b.z; g[4 * h + 3] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int e = (j >> 2) * 128 + lane * 4 + (j & 3);
+            th[j] = e < n ? tp[e] : 0.f;  // behind the tensor's end: the padding, whose codes stay 0
+            g[j] = e < n ? gp[e] : 0.f;
+        }
+    }
     float mn[8], root[8];
+    uint32_t cm[2], cv[2];
+    float um = 0.f, ur = 0.f;
+    if (!k.first) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            cm[h] = mc[s / 4 + h * 32 + lane];
+            cv[h] = vc[s / 4 + h * 32 + lane];
+        }
+        um = ms[block] * (1.f / (M_TOP * M_TOP));
+        ur = vs[block] * (1.f / (V_TOP * V_TOP));
+    }
+    const Pair<float> mz = pair(minus_zero, minus_zero);
+    auto times = [&](const Pair<float>& x, const Pair<float>& y) { return rounded_product(x, y, mz); };
+    // adam_one's chain without its additions of 0 (they only turn -0 into 0), two elements at a time
+    const Pair<float> b1 = pair(k.b1, k.b1), omb1 = pair(k.omb1, k.omb1), b2 = pair(k.b2, k.b2), omb2 = pair(k.omb2, k.omb2);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        Pair<float> a = pair(th[j], th[j + 1]), gr = pair(g[j], g[j + 1]);
+        if (k.scale_grad) gr = times(gr, pair(k.gscale, k.gscale));
+        if (k.has_wd) {
+            if (k.decoupled) a = times(a, pair(k.decay_mul, k.decay_mul));
+            else gr = gr + times(a, pair(k.wd, k.wd));
+        }
+        Pair<float> m = times(gr, omb1), v = times(times(gr, gr), omb2);
+        if (!k.first) {
+            const Pair<float> old = pair(decode_m(m_code(cm[j >> 2], j & 3), um), decode_m(m_code(cm[j >> 2], (j & 3) + 1), um));
+            const Pair<float> c = pair(v_code(cv[j >> 2], j & 3), v_code(cv[j >> 2], (j & 3) + 1));
+            const Pair<float> r = times(times(c, c), pair(ur, ur));
+            m = times(old, b1) + m;
+            v = times(times(r, r), b2) + v;
+        }
+        float v0, v1, d0, d1;
+        unpair(m, mn[j], mn[j + 1]);
+        unpair(v, v0, v1);
+        root[j] = sqrtf(v0);
+        root[j + 1] = sqrtf(v1);
+        unpair(times(pair(root[j], root[j + 1]), pair(k.inv_sqrt_bc2, k.inv_sqrt_bc2)) + pair(k.eps, k.eps), d0, d1);
+        unpair(a + times(pair(mn[j] / d0, mn[j + 1] / d1), pair(-k.step_size, -k.step_size)), th[j], th[j + 1]);
+    }
+    if (wide) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<float4*>(tp + h * 128 + lane * 4) = make_float4(th[4 * h], th[4 * h + 1], th[4 * h + 2], th[4 * h + 3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int e = (j >> 2) * 128 + lane * 4 + (j & 3);
+            if (e < n) tp[e] = th[j];
+            else mn[j] = root[j] = 0.f;
+        }
+    }
     unsigned int top_m = 0, top_r = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const int e = j * 32 + lane;
-        float vi = 0.f;
-        mn[j] = 0.f;
-        root[j] = 0.f;
-        if (at + e < len) {
-            float th = t.theta[at + e];
-            if (!k.first) {
-                mn[j] = decode_m(mc[s + e], um);
-                const float r = decode_root(vc[s + e], ur);
-                vi = r * r;
-            }
-            adam_one(th, t.grad[at + e], mn[j], vi, kt);
-            t.theta[at + e] = th;
-            root[j] = sqrtf(vi);
-        }
-        top_m = max(top_m, __float_as_uint(fabsf(mn[j])));
+        top_m = max(top_m, __float_as_uint(mn[j]) & 0x7fffffffu);
         top_r = max(top_r, __float_as_uint(root[j]) & 0x7fffffffu);
     }
     const float sm = block_scale(__reduce_max_sync(0xffffffffu, top_m)), sr = block_scale(__reduce_max_sync(0xffffffffu, top_r));
-    const float lm = (M_TOP * M_TOP) / sm, lr = (V_TOP * V_TOP) / sr;
+    float mag[8];
+    uint32_t code[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int e = j * 32 + lane;  // behind the tensor's end: the padding, whose codes are 0
-        const int c = encode(fabsf(mn[j]), lm, M_TOP), r = encode(root[j], lr, V_TOP);
-        mc[s + e] = static_cast<int8_t>(mn[j] < 0.f ? -c : c);
-        vc[s + e] = static_cast<uint8_t>(root[j] > 0.f ? max(r, 1) : r);
-    }
+    for (int j = 0; j < 8; ++j) mag[j] = fabsf(mn[j]);
+    encode(mag, (M_TOP * M_TOP) / sm, M_TOP, code);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (mn[j] < 0.f) code[j] = 0u - code[j];  // the low byte of -(2^23 + c) is that of -c
+#pragma unroll
+    for (int h = 0; h < 2; ++h) mc[s / 4 + h * 32 + lane] = pack_bytes(code[4 * h], code[4 * h + 1], code[4 * h + 2], code[4 * h + 3]);
+    encode(root, (V_TOP * V_TOP) / sr, V_TOP, code);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (root[j] > 0.f) code[j] = max(code[j], 0x4B000001u);  // what is not zero stays so
+#pragma unroll
+    for (int h = 0; h < 2; ++h) vc[s / 4 + h * 32 + lane] = pack_bytes(code[4 * h], code[4 * h + 1], code[4 * h + 2], code[4 * h + 3]);
     if (lane == 0) {
         ms[block] = sm;
         vs[block] = sr;
     }
 }
 
-// The values that the 8-bit state stands for.
-__global__ void __launch_bounds__(THREADS) adam_multi8_read_kernel(const int8_t* __restrict__ mc, const uint8_t* __restrict__ vc,
+// The values that the 8-bit state stands for, four at a time (the state's length is a multiple of 256).
+__global__ void __launch_bounds__(THREADS) adam_multi8_read_kernel(const uint32_t* __restrict__ mc, const uint32_t* __restrict__ vc,
                                                                    const float* __restrict__ ms, const float* __restrict__ vs, float* __restrict__ m,
-                                                                   float* __restrict__ v, int64_t n) {
+                                                                   float* __restrict__ v, int64_t groups, int wide) {
     wb_pdl_enter();
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
-    if (i >= n) return;
-    if (m) m[i] = decode_m(mc[i], ms[i / BLOCK8] * (1.f / (M_TOP * M_TOP)));
+    const int64_t q = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+    if (q >= groups) return;
+    auto put = [&](float* to, const float (&a)[4]) {
+        if (wide) {
+            reinterpret_cast<float4*>(to)[q] = make_float4(a[0], a[1], a[2], a[3]);
+        } else {
+            for (int i = 0; i < 4; ++i) to[4 * q + i] = a[i];
+        }
+    };
+    float a[4];
+    if (m) {
+        const uint32_t c = mc[q];
+        const float unit = ms[q / (BLOCK8 / 4)] * (1.f / (M_TOP * M_TOP));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = decode_m(m_code(c, i), unit);
+        put(m, a);
+    }
     if (v) {
-        const float r = decode_root(vc[i], vs[i / BLOCK8] * (1.f / (V_TOP * V_TOP)));
-        v[i] = r * r;
+        const uint32_t c = vc[q];
+        const float unit = vs[q / (BLOCK8 / 4)] * (1.f / (V_TOP * V_TOP));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float r = decode_root(v_code(c, i), unit);
+            a[i] = r * r;
+        }
+        put(v, a);
     }
 }
 
 // ---- the norm -----------------------------------------------------------------------------------------------
 
 // Squares of f32 are exact in f64 and neither overflow nor vanish there; sums in f64, each in a fixed order.  Block b of
-// this launch takes chunks b, b + gridDim, ... and leaves parts[at + b]; the block that arrives last of all launches
-// joins the `total` parts and leaves the counter zero.
+// this launch takes its share of the chunks, one after the other (so that it looks the first one's tensor up and then walks on),
+// and leaves parts[at + b]; the block that arrives last of all launches joins the `total` parts and leaves the counter zero.
 template <int N>
 __global__ void __launch_bounds__(THREADS) grad_norm_kernel(const __grid_constant__ Table<N> tab, double* __restrict__ parts, int at, int total,
                                                             unsigned int* __restrict__ counter, double max_norm, float* __restrict__ norm,
@@ -182,16 +328,41 @@ __global__ void __launch_bounds__(THREADS) grad_norm_kernel(const __grid_constan
     __shared__ double warp_sum[THREADS / 32];
     __shared__ unsigned int last;
     wb_pdl_enter();
+    unsigned int c = static_cast<unsigned int>(static_cast<uint64_t>(tab.chunks) * blockIdx.x / gridDim.x);
+    const unsigned int end = static_cast<unsigned int>(static_cast<uint64_t>(tab.chunks) * (blockIdx.x + 1) / gridDim.x);
     double acc = 0.0;
-    for (unsigned int c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-        const int ti = find_tensor(tab, c);
+    auto add = [&](float g) {
+        const double d = g;
+        acc += d * d;
+    };
+    for (int ti = c < end ? find_tensor(tab, c) : 0; c < end; ++ti) {
         const Tensor& t = tab.t[ti];
-        if (!t.grad) continue;
-        const int64_t len = t.len < 0 ? -t.len : t.len, i0 = static_cast<int64_t>(c - tab.first[ti]) * CHUNK, end = min(i0 + CHUNK, len);
-        for (int64_t i = i0 + threadIdx.x; i < end; i += THREADS) {
-            const double g = t.grad[i];
-            acc += g * g;
+        const unsigned int next = ti + 1 < tab.n ? min(tab.first[ti + 1], end) : end;
+        if (next <= c) continue;  // a tensor of no chunk
+        if (t.grad) {
+            const int64_t len = t.len < 0 ? -t.len : t.len;
+            const int64_t i0 = static_cast<int64_t>(c - tab.first[ti]) * CHUNK, i1 = min(static_cast<int64_t>(next - tab.first[ti]) * CHUNK, len);
+            const float* g = t.grad + i0;
+            const int64_t n = i1 - i0, head = min(n, static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) / 4);
+            const int64_t packs = (n - head) / 4;
+            if (threadIdx.x < head) add(g[threadIdx.x]);
+            const float4* g4 = reinterpret_cast<const float4*>(g + head);
+            for (int64_t q0 = threadIdx.x; q0 < packs; q0 += 4 * THREADS) {
+                float4 a[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) a[u] = q0 + u * THREADS < packs ? g4[q0 + u * THREADS] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    add(a[u].x);
+                    add(a[u].y);
+                    add(a[u].z);
+                    add(a[u].w);
+                }
+            }
+            const int64_t rest = head + 4 * packs + threadIdx.x;
+            if (rest < n) add(g[rest]);
         }
+        c = next;
     }
     auto block_sum = [&](double v) {
 #pragma unroll
@@ -436,8 +607,8 @@ extern "C" int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64
             WB_CHECK_CUDA(wb_launch_pdl(adam_multi32_kernel<N>, dim3(tab.chunks), dim3(THREADS), 0, b->stream, tab, m, m + p, k, device_grad_scale));
         } else {
             float* scales = reinterpret_cast<float*>(h->state + 2 * p);
-            WB_CHECK_CUDA(wb_launch_pdl(adam_multi8_kernel<N>, dim3(tab.chunks), dim3(THREADS), 0, b->stream, tab, reinterpret_cast<int8_t*>(h->state),
-                                        reinterpret_cast<uint8_t*>(h->state + p), scales, scales + p / BLOCK8, k, device_grad_scale));
+            WB_CHECK_CUDA(wb_launch_pdl(adam_multi8_kernel<N>, dim3(tab.chunks), dim3(THREADS), 0, b->stream, tab, reinterpret_cast<uint32_t*>(h->state),
+                                        reinterpret_cast<uint32_t*>(h->state + p), scales, scales + p / BLOCK8, k, device_grad_scale, -0.f));
         }
         WB_LAUNCH_OK(b);
         return WB_OK;
@@ -465,10 +636,12 @@ extern "C" int wb_adam_multi_read_state(WbAdamMulti* h, float* m, float* v) {
         return WB_OK;
     }
     const float* scales = reinterpret_cast<const float*>(state + 2 * p);
-    const int64_t grid = (p + THREADS - 1) / THREADS;
+    const int64_t groups = p / 4, grid = (groups + THREADS - 1) / THREADS;
     WB_REQUIRE(grid <= INT32_MAX, WB_ERR_INVALID, "wb_adam_multi_read_state: state too large");
+    const int wide = ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
     WB_CHECK_CUDA(wb_launch_pdl(adam_multi8_read_kernel, dim3(static_cast<unsigned>(grid)), dim3(THREADS), 0, b->stream,
-                                reinterpret_cast<const int8_t*>(state), reinterpret_cast<const uint8_t*>(state + p), scales, scales + p / BLOCK8, m, v, p));
+                                reinterpret_cast<const uint32_t*>(state), reinterpret_cast<const uint32_t*>(state + p), scales, scales + p / BLOCK8, m, v,
+                                groups, wide));
     WB_LAUNCH_OK(b);
     return WB_OK;
 }
