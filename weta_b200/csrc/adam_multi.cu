@@ -13,6 +13,7 @@
 // codes do not depend on the launch's shape, and the 32-bit step gives wb_adam_step's bits.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <new>
 
 #include "adam.cuh"
@@ -23,7 +24,7 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int BLOCK8 = 256;        // elements that share a scale: one warp, eight per lane
-constexpr int64_t CHUNK = 2048;    // elements a thread block takes at a time, all of one tensor
+constexpr int CHUNK = 2048;         // elements a thread block takes at a time, all of one tensor
 constexpr float M_TOP = 127.f, V_TOP = 255.f;
 constexpr float TINY = 7.8886090522101181e-31f;  // 2^-100, the least scale: its reciprocal is still finite
 
@@ -34,20 +35,25 @@ struct Tensor {
     int64_t len;  // negative: -len elements, exempt from weight decay
 };
 
+constexpr int HINTS = 128;
+
 // The tensors of one launch, passed by value: nothing to upload, nothing a captured graph could lose.
 template <int N>
 struct Table {
     int n;
-    unsigned int chunks;          // of all tensors together
-    unsigned int first[N];        // a tensor's first chunk
+    int shift;
+    unsigned int chunks;    // of all tensors together
+    uint16_t hint[HINTS + 1];  // the tensor of chunk i << shift
+    unsigned int first[N];  // a tensor's first chunk
     Tensor t[N];
 };
 
 // The tensor that holds chunk c: the last one whose first chunk is not behind it (tensors of no chunk share their
-// successor's first one).
+// successor's first one).  Between two hints few are left to search: every step is a dependent load that the block's first
+// load of data waits for.
 template <int N>
 __device__ __forceinline__ int find_tensor(const Table<N>& tab, unsigned int c) {
-    int lo = 0, hi = tab.n - 1;
+    int lo = tab.hint[c >> tab.shift], hi = tab.hint[(c >> tab.shift) + 1];
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (tab.first[mid] <= c) lo = mid;
@@ -89,9 +95,9 @@ __global__ void __launch_bounds__(THREADS) adam_multi32_kernel(const __grid_cons
     if (t.len < 0) k.has_wd = 0;
     float *th = t.theta + at, *mp = m + t.offset + at, *vp = v + t.offset + at;
     const float* gp = t.grad + at;
-    const int n = static_cast<int>(min(CHUNK, len - at));
+    const int n = static_cast<int>(min(static_cast<int64_t>(CHUNK), len - at));
     if (((reinterpret_cast<uintptr_t>(t.theta) | reinterpret_cast<uintptr_t>(t.grad)) & 15) == 0) {
-        constexpr int U = static_cast<int>(CHUNK) / (4 * THREADS);
+        constexpr int U = CHUNK / (4 * THREADS);
         float4 a[U], g[U], mi[U], vi[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -126,85 +132,161 @@ __global__ void __launch_bounds__(THREADS) adam_multi32_kernel(const __grid_cons
 // ---- 8-bit state --------------------------------------------------------------------------------------------
 
 // A byte as f32 without the conversion unit (16 lanes per clock, which the square roots and the division need): put under
-// the exponent of 2^23 it is 2^23 + byte, exactly; and a value in [0, 255] plus 2^23 is rounded to the nearest integer, ties
-// to even, which then is the low byte.
-constexpr float MAGIC = 8388608.f;
-__device__ __forceinline__ float byte_of(uint32_t word, int i, float minus) { return __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7440 + i)) + minus; }
-__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+// the exponent of 2^23 it is 2^23 + byte, exactly.  And a value of magnitude under 2^22 plus 1.5 * 2^23 is rounded to the
+// nearest integer, ties to even, whose two's complement the low bits then are.
+constexpr float BYTE_BASE = 8388608.f, MAGIC = 12582912.f;
+__device__ __forceinline__ float based_byte(uint32_t word, int i) { return __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7440 + i)); }
+__device__ __forceinline__ Pair<float> bytes_of(uint32_t word, int i, float base) {
+    return pair(based_byte(word, i), based_byte(word, i + 1)) + pair(-base, -base);
 }
-// c |c| unit and (c c unit)^2 for the values c of the codes.
+// The codes' values; codes of m are signed.
+__device__ __forceinline__ Pair<float> m_codes(uint32_t word, int i) { return bytes_of(word ^ 0x80808080u, i, BYTE_BASE + 128.f); }
+__device__ __forceinline__ Pair<float> v_codes(uint32_t word, int i) { return bytes_of(word, i, BYTE_BASE); }
+__device__ __forceinline__ uint32_t pack_bytes(const uint32_t* c) {
+    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
 __device__ __forceinline__ float decode_m(float c, float unit) { return c * fabsf(c) * unit; }
 __device__ __forceinline__ float decode_root(float c, float unit) { return c * c * unit; }
-__device__ __forceinline__ float m_code(uint32_t word, int i) { return byte_of(word ^ 0x80808080u, i, -(MAGIC + 128.f)); }
-__device__ __forceinline__ float v_code(uint32_t word, int i) { return byte_of(word, i, -MAGIC); }
 
-// The scale of a block whose largest magnitude has these bits.  One that is not finite poisons the block: its scale is
-// stored as NaN, and every value read from it is NaN.
-__device__ __forceinline__ float block_scale(unsigned int bits) {
+// Square root and quotient, correctly rounded, two at a time, for operands far from the ends of the exponent range (the
+// caller sends all others to sqrtf and /): an approximation from the function unit, refined, then corrected by its exact
+// residual with one fused operation (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", IBM J. Res. Dev. 34, 1990: with 1/d correctly rounded and q within a unit, q + (m - d q) / d rounds to m/d).
+// That the reciprocal is correctly rounded, and the root, was checked for every mantissa (and both parities of the exponent).
+__device__ __forceinline__ Pair<float> root_of(const Pair<float>& v) {
+    float a, b, ya, yb;
+    unpair(v, a, b);
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(ya) : "f"(a));
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(yb) : "f"(b));
+    const Pair<float> y = pair(ya, yb), g = v * y, minus_v = v * pair(-1.f, -1.f), minus_half = y * pair(-0.5f, -0.5f);
+    return muladd(muladd(g, g, minus_v), minus_half, g);
+}
+// m / d from -d.
+__device__ __forceinline__ Pair<float> quotient_of(const Pair<float>& m, const Pair<float>& minus_d) {
+    float a, b, ya, yb;
+    unpair(minus_d, a, b);
+    asm("rcp.approx.f32 %0, %1;" : "=f"(ya) : "f"(-a));
+    asm("rcp.approx.f32 %0, %1;" : "=f"(yb) : "f"(-b));
+    Pair<float> y = pair(ya, yb);
+    y = muladd(muladd(minus_d, y, pair(1.f, 1.f)), y, y);
+    const Pair<float> q = m * y;
+    return muladd(muladd(minus_d, q, m), y, q);
+}
+
+// The largest and the least of three magnitudes; `largest_or_nan` is NaN if one is.
+__device__ __forceinline__ float largest_or_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float largest(float a, float b, float c) {
+    float r;
+    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float least(float a, float b, float c) {
+    float r;
+    asm("min.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// The scale of a block from every lane's largest magnitude.  One that is not finite poisons the block: its scale is stored as
+// NaN, and every value read from it is NaN.  (The bits of f32 magnitudes order like the values, NaN last.)
+__device__ __forceinline__ float block_scale(float lane_max) {
+    const unsigned int bits = __reduce_max_sync(0xffffffffu, __float_as_uint(lane_max) & 0x7fffffffu);
     if (bits >= 0x7f800000u) return __int_as_float(0x7fffffff);
     return fmaxf(__uint_as_float(bits), TINY);
 }
 
-// Codes of eight magnitudes: min(rint(sqrt(x level)), top), the square root correctly rounded.  The approximate one is off by
-// less than 2^-20 of at most 256, which moves rint's result only next to a half: a lane that comes within 2^-11 of one
-// takes all its roots again.  Each result is 2^23 + code.
-__device__ __forceinline__ void encode(const float (&x)[8], float level, float top, uint32_t (&code)[8]) {
-    float far = 0.f;
+// Codes of eight values: rint(sqrt(|x| level)), the square root correctly rounded; negative where x is (SIGNED); at least 1
+// where x is above 0 (else).  level is top^2 / (largest |x|), so sqrt(|x| level) exceeds top by rounding at most and no code
+// does.  The approximate square root's relative error is at most 2^-23 (PTX ISA, sqrt.approx), 2^-15 of at most 256, and moves
+// rint's result only next to a half: a lane that comes within 2^-14 of one takes all its roots again (within 2^-11, every
+// fourth warp did).  The codes are the results' low bytes.
+template <bool SIGNED>
+__device__ __forceinline__ void encode(const Pair<float> (&x)[4], float level, uint32_t (&code)[8]) {
+    float far = 0.f, low = 1.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float s;
-        asm("sqrt.approx.f32 %0, %1;" : "=f"(s) : "f"(x[j] * level));
-        s = fminf(s, top);
-        const float r = s + MAGIC;
-        far = fmaxf(far, fabsf(s - (r - MAGIC)));
-        code[j] = __float_as_uint(r);
+    for (int j = 0; j < 4; ++j) {
+        float q0, q1, s0, s1, f0, f1, c0, c1;
+        unpair(x[j] * pair(level, level), q0, q1);
+        asm("sqrt.approx.f32 %0, %1;" : "=f"(s0) : "f"(fabsf(q0)));
+        asm("sqrt.approx.f32 %0, %1;" : "=f"(s1) : "f"(fabsf(q1)));
+        if (!SIGNED) low = least(low, s0, s1);
+        const Pair<float> s = SIGNED ? pair(copysignf(s0, q0), copysignf(s1, q1)) : pair(s0, s1), r = s + pair(MAGIC, MAGIC);
+        unpair(s + muladd(r, pair(-1.f, -1.f), pair(MAGIC, MAGIC)), f0, f1);
+        far = largest(far, f0, f1);
+        unpair(r, c0, c1);
+        code[2 * j] = __float_as_uint(c0);
+        code[2 * j + 1] = __float_as_uint(c1);
     }
-    if (far > 0.49951171875f) {
+    if (far > 0.49993896484375f || (!SIGNED && low < 1.f)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) code[j] = __float_as_uint(fminf(sqrtf(x[j] * level), top) + MAGIC);
+        for (int j = 0; j < 8; ++j) {
+            float a, b;
+            unpair(x[j >> 1], a, b);
+            if (j & 1) a = b;
+            float s = sqrtf(fabsf(a * level));
+            s = SIGNED ? copysignf(s, a) : fmaxf(s, a > 0.f ? 1.f : 0.f);
+            code[j] = __float_as_uint(s + MAGIC);
+        }
     }
 }
 
+// The step's scalars, each twice, so that a packed operation reads both from the constant bank at once.
+struct AdamK8 {
+    Pair<float> b1, omb1, b2, omb2, minus_inv_sqrt_bc2, minus_eps, minus_step, minus_zero;
+    float gscale, decay_mul;  // 1 where there is none: x * 1 is x
+    float wd, inv_sqrt_bc2, eps, step;
+    int l2;          // weight decay through the gradient
+    int eps_normal;  // eps is at least 2^-60
+};
+
 // One warp takes a block of 256 elements, a lane the groups of four at 4 lane and 128 + 4 lane.
-template <int N>
-__global__ void __launch_bounds__(THREADS) adam_multi8_kernel(const __grid_constant__ Table<N> tab, uint32_t* __restrict__ mc, uint32_t* __restrict__ vc,
-                                                              float* __restrict__ ms, float* __restrict__ vs, AdamK k0,
-                                                              const float* __restrict__ scale, float minus_zero) {
+// Bound by instruction issue until the conversions left the conversion unit, the arithmetic went to pairs and a block took
+// a longer chunk (101 M elements in 128 tensors: 562 -> 293 us).
+template <int N, bool FIRST>
+__global__ void __launch_bounds__(THREADS, 5) adam_multi8_kernel(const __grid_constant__ Table<N> tab, uint32_t* __restrict__ mc, uint32_t* __restrict__ vc,
+                                                              float* __restrict__ ms, float* __restrict__ vs, const __grid_constant__ AdamK8 k8,
+                                                              const float* __restrict__ scale) {
     wb_pdl_enter();
     const int ti = find_tensor(tab, blockIdx.x);
     const Tensor t = tab.t[ti];
     if (!t.grad) return;
     const int64_t len = t.len < 0 ? -t.len : t.len;
-    const int64_t at = static_cast<int64_t>(blockIdx.x - tab.first[ti]) * CHUNK + (threadIdx.x >> 5) * BLOCK8;
-    if (at >= len) return;
-    AdamK k = with_device_scale(k0, scale);
-    if (t.len < 0) k.has_wd = 0;
-    const int lane = threadIdx.x & 31, n = static_cast<int>(min(static_cast<int64_t>(BLOCK8), len - at));
-    const int64_t s = t.offset + at, block = s / BLOCK8;
-    float* tp = t.theta + at;
-    const float* gp = t.grad + at;
-    float th[8], g[8];
-    const bool wide = n == BLOCK8 && ((reinterpret_cast<uintptr_t>(t.theta) | reinterpret_cast<uintptr_t>(t.grad)) & 15) == 0;
+    const float gscale = scale ? k8.gscale * *scale : k8.gscale, shrink = t.len < 0 ? 1.f : k8.decay_mul;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(t.theta) | reinterpret_cast<uintptr_t>(t.grad)) & 15) == 0;
+    const int lane = threadIdx.x & 31;
+    const int64_t start = static_cast<int64_t>(blockIdx.x - tab.first[ti]) * CHUNK + (threadIdx.x >> 5) * BLOCK8;
+    if (start >= len) return;
+    const int n = static_cast<int>(min(static_cast<int64_t>(BLOCK8), len - start));
+    // x y, rounded whatever is added to it (see rounded_product)
+    auto times = [&](const Pair<float>& x, const Pair<float>& y) { return rounded_product(x, y, k8.minus_zero); };
+    const int64_t s = t.offset + start, block = s / BLOCK8;
+    float* tp = t.theta + start;
+    const float* gp = t.grad + start;
+    Pair<float> th[4], g[4], mn[4], root[4];  // root: first v
+    const bool wide = aligned && n == BLOCK8;
+    auto at = [&](int j) { return (j >> 1) * 128 + lane * 4 + 2 * (j & 1); };  // pair j's place in the block
     if (wide) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const float4 a = *reinterpret_cast<const float4*>(tp + h * 128 + lane * 4), b = *reinterpret_cast<const float4*>(gp + h * 128 + lane * 4);
-            th[4 * h] = a.x; th[4 * h + 1] = a.y; th[4 * h + 2] = a.z; th[4 * h + 3] = a.w;
-            g[4 * h] = b.x; g[4 * h + 1] = b.y; g[4 * h + 2] = b.z; g[4 * h + 3] = b.w;
+            const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(tp + at(2 * h)), b = *reinterpret_cast<const ulonglong2*>(gp + at(2 * h));
+            th[2 * h].v = a.x;
+            th[2 * h + 1].v = a.y;
+            g[2 * h].v = b.x;
+            g[2 * h + 1].v = b.y;
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int e = (j >> 2) * 128 + lane * 4 + (j & 3);
-            th[j] = e < n ? tp[e] : 0.f;  // behind the tensor's end: the padding, whose codes stay 0
-            g[j] = e < n ? gp[e] : 0.f;
+        for (int j = 0; j < 4; ++j) {
+            const int e = at(j);
+            th[j] = pair(e < n ? tp[e] : 0.f, e + 1 < n ? tp[e + 1] : 0.f);
+            g[j] = pair(e < n ? gp[e] : 0.f, e + 1 < n ? gp[e + 1] : 0.f);
         }
     }
-    float mn[8], root[8];
     uint32_t cm[2], cv[2];
     float um = 0.f, ur = 0.f;
-    if (!k.first) {
+    if (!FIRST) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             cm[h] = mc[s / 4 + h * 32 + lane];
@@ -213,69 +295,89 @@ __global__ void __launch_bounds__(THREADS) adam_multi8_kernel(const __grid_const
         um = ms[block] * (1.f / (M_TOP * M_TOP));
         ur = vs[block] * (1.f / (V_TOP * V_TOP));
     }
-    const Pair<float> mz = pair(minus_zero, minus_zero);
-    auto times = [&](const Pair<float>& x, const Pair<float>& y) { return rounded_product(x, y, mz); };
     // adam_one's chain without its additions of 0 (they only turn -0 into 0), two elements at a time
-    const Pair<float> b1 = pair(k.b1, k.b1), omb1 = pair(k.omb1, k.omb1), b2 = pair(k.b2, k.b2), omb2 = pair(k.omb2, k.omb2);
+    const Pair<float> by = pair(gscale, gscale), keep = pair(shrink, shrink);
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        Pair<float> a = pair(th[j], th[j + 1]), gr = pair(g[j], g[j + 1]);
-        if (k.scale_grad) gr = times(gr, pair(k.gscale, k.gscale));
-        if (k.has_wd) {
-            if (k.decoupled) a = times(a, pair(k.decay_mul, k.decay_mul));
-            else gr = gr + times(a, pair(k.wd, k.wd));
+    for (int j = 0; j < 4; ++j) g[j] = times(g[j], by);
+    if (k8.l2 && t.len >= 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) g[j] = g[j] + times(th[j], pair(k8.wd, k8.wd));
+    }
+    float top_m = 0.f, top_v = 0.f, low_m = 1.f, low_v = 1.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        Pair<float> m = times(g[j], k8.omb1), v = times(times(g[j], g[j]), k8.omb2);
+        if (!FIRST) {
+            float c0, c1;
+            unpair(m_codes(cm[j >> 1], 2 * (j & 1)), c0, c1);
+            const Pair<float> old = times(pair(c0 * fabsf(c0), c1 * fabsf(c1)), pair(um, um));
+            const Pair<float> c = v_codes(cv[j >> 1], 2 * (j & 1)), r = times(times(c, c), pair(ur, ur));
+            m = times(old, k8.b1) + m;
+            v = times(times(r, r), k8.b2) + v;
         }
-        Pair<float> m = times(gr, omb1), v = times(times(gr, gr), omb2);
-        if (!k.first) {
-            const Pair<float> old = pair(decode_m(m_code(cm[j >> 2], j & 3), um), decode_m(m_code(cm[j >> 2], (j & 3) + 1), um));
-            const Pair<float> c = pair(v_code(cv[j >> 2], j & 3), v_code(cv[j >> 2], (j & 3) + 1));
-            const Pair<float> r = times(times(c, c), pair(ur, ur));
-            m = times(old, b1) + m;
-            v = times(times(r, r), b2) + v;
+        if (n < BLOCK8) {  // behind the tensor's end: the padding, whose codes stay 0
+            if (at(j) >= n) m = v = pair(0.f, 0.f);
+            else if (at(j) + 1 >= n) {
+                float a, b;
+                unpair(m, a, b);
+                m = pair(a, 0.f);
+                unpair(v, a, b);
+                v = pair(a, 0.f);
+            }
         }
-        float v0, v1, d0, d1;
-        unpair(m, mn[j], mn[j + 1]);
-        unpair(v, v0, v1);
-        root[j] = sqrtf(v0);
-        root[j + 1] = sqrtf(v1);
-        unpair(times(pair(root[j], root[j + 1]), pair(k.inv_sqrt_bc2, k.inv_sqrt_bc2)) + pair(k.eps, k.eps), d0, d1);
-        unpair(a + times(pair(mn[j] / d0, mn[j + 1] / d1), pair(-k.step_size, -k.step_size)), th[j], th[j + 1]);
+        th[j] = times(th[j], keep);
+        mn[j] = m;
+        root[j] = v;
+        float a, b;
+        unpair(m, a, b);
+        top_m = largest_or_nan(top_m, a, b);
+        low_m = least(low_m, a, b);
+        unpair(v, a, b);
+        top_v = largest_or_nan(top_v, a, b);
+        low_v = least(low_v, a, b);
+    }
+    // m in [2^-60, 2^60], v in [2^-100, 2^120] and eps at least 2^-60: nothing below leaves the normal range
+    if (k8.eps_normal && low_m >= 8.6736173798840355e-19f && low_v >= 7.8886090522101181e-31f && top_m <= 1.152921504606847e18f &&
+        top_v <= 1.3292279957849159e36f) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            root[j] = root_of(root[j]);
+            th[j] = th[j] + times(quotient_of(mn[j], times(root[j], k8.minus_inv_sqrt_bc2) + k8.minus_eps), k8.minus_step);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float m0, m1, r0, r1, t0, t1;
+            unpair(mn[j], m0, m1);
+            unpair(root[j], r0, r1);
+            unpair(th[j], t0, t1);
+            r0 = sqrtf(r0);
+            r1 = sqrtf(r1);
+            root[j] = pair(r0, r1);
+            th[j] = pair(t0 - m0 / (r0 * k8.inv_sqrt_bc2 + k8.eps) * k8.step, t1 - m1 / (r1 * k8.inv_sqrt_bc2 + k8.eps) * k8.step);
+        }
     }
     if (wide) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<float4*>(tp + h * 128 + lane * 4) = make_float4(th[4 * h], th[4 * h + 1], th[4 * h + 2], th[4 * h + 3]);
+        for (int h = 0; h < 2; ++h) *reinterpret_cast<ulonglong2*>(tp + at(2 * h)) = make_ulonglong2(th[2 * h].v, th[2 * h + 1].v);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int e = (j >> 2) * 128 + lane * 4 + (j & 3);
-            if (e < n) tp[e] = th[j];
-            else mn[j] = root[j] = 0.f;
+        for (int j = 0; j < 4; ++j) {
+            float a, b;
+            unpair(th[j], a, b);
+            if (at(j) < n) tp[at(j)] = a;
+            if (at(j) + 1 < n) tp[at(j) + 1] = b;
         }
     }
-    unsigned int top_m = 0, top_r = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        top_m = max(top_m, __float_as_uint(mn[j]) & 0x7fffffffu);
-        top_r = max(top_r, __float_as_uint(root[j]) & 0x7fffffffu);
-    }
-    const float sm = block_scale(__reduce_max_sync(0xffffffffu, top_m)), sr = block_scale(__reduce_max_sync(0xffffffffu, top_r));
-    float mag[8];
+    // the largest root is the root of the largest v: rounding is monotone
+    const float sm = block_scale(top_m), sr = block_scale(sqrtf(top_v));
     uint32_t code[8];
+    encode<true>(mn, (M_TOP * M_TOP) / sm, code);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) mag[j] = fabsf(mn[j]);
-    encode(mag, (M_TOP * M_TOP) / sm, M_TOP, code);
+    for (int h = 0; h < 2; ++h) mc[s / 4 + h * 32 + lane] = pack_bytes(code + 4 * h);
+    encode<false>(root, (V_TOP * V_TOP) / sr, code);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (mn[j] < 0.f) code[j] = 0u - code[j];  // the low byte of -(2^23 + c) is that of -c
-#pragma unroll
-    for (int h = 0; h < 2; ++h) mc[s / 4 + h * 32 + lane] = pack_bytes(code[4 * h], code[4 * h + 1], code[4 * h + 2], code[4 * h + 3]);
-    encode(root, (V_TOP * V_TOP) / sr, V_TOP, code);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (root[j] > 0.f) code[j] = max(code[j], 0x4B000001u);  // what is not zero stays so
-#pragma unroll
-    for (int h = 0; h < 2; ++h) vc[s / 4 + h * 32 + lane] = pack_bytes(code[4 * h], code[4 * h + 1], code[4 * h + 2], code[4 * h + 3]);
+    for (int h = 0; h < 2; ++h) vc[s / 4 + h * 32 + lane] = pack_bytes(code + 4 * h);
     if (lane == 0) {
         ms[block] = sm;
         vs[block] = sr;
@@ -301,16 +403,23 @@ __global__ void __launch_bounds__(THREADS) adam_multi8_read_kernel(const uint32_
         const uint32_t c = mc[q];
         const float unit = ms[q / (BLOCK8 / 4)] * (1.f / (M_TOP * M_TOP));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = decode_m(m_code(c, i), unit);
+        for (int i = 0; i < 4; i += 2) {
+            unpair(m_codes(c, i), a[i], a[i + 1]);
+            a[i] = decode_m(a[i], unit);
+            a[i + 1] = decode_m(a[i + 1], unit);
+        }
         put(m, a);
     }
     if (v) {
         const uint32_t c = vc[q];
         const float unit = vs[q / (BLOCK8 / 4)] * (1.f / (V_TOP * V_TOP));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float r = decode_root(v_code(c, i), unit);
-            a[i] = r * r;
+        for (int i = 0; i < 4; i += 2) {
+            unpair(v_codes(c, i), a[i], a[i + 1]);
+            a[i] = decode_root(a[i], unit);
+            a[i + 1] = decode_root(a[i + 1], unit);
+            a[i] *= a[i];
+            a[i + 1] *= a[i + 1];
         }
         put(v, a);
     }
@@ -398,8 +507,8 @@ __global__ void __launch_bounds__(THREADS) grad_norm_kernel(const __grid_constan
 
 // ---- the handle ---------------------------------------------------------------------------------------------
 
-constexpr int SMALL = 32, LARGE = 768;  // tensors per launch: 1.2 KB and 28 KB of parameters (limit: 32,764 bytes)
-static_assert(sizeof(Table<LARGE>) + 128 <= 32764, "a launch's parameters");
+constexpr int SMALL = 32, LARGE = 768;  // tensors per launch: 1.5 KB and 28 KB of parameters (limit: 32,764 bytes)
+static_assert(sizeof(Table<LARGE>) + sizeof(AdamK8) + 64 <= 32764, "a launch's parameters");
 
 int64_t padded(int64_t n) { return (n + BLOCK8 - 1) / BLOCK8 * BLOCK8; }
 int64_t chunks_of(int64_t len) { return (len + CHUNK - 1) / CHUNK; }
@@ -445,7 +554,9 @@ int per_launch(WbAdamMulti* h, F&& launch) {
         if (t.n <= SMALL) {
             Table<SMALL> s;
             s.n = t.n;
+            s.shift = t.shift;
             s.chunks = t.chunks;
+            std::copy(t.hint, t.hint + HINTS + 1, s.hint);
             std::copy(t.first, t.first + t.n, s.first);
             std::copy(t.t, t.t + t.n, s.t);
             WB_TRY(launch(static_cast<int>(l), s));
@@ -485,6 +596,7 @@ int create(WbBackend* b, const WbAdamTensor* tensors, int n, int state_bits, voi
         if (h->launches.empty() || h->launches.back().n == LARGE || h->launches.back().chunks + chunks_of(h->lens[i]) > INT32_MAX) {
             h->launches.emplace_back();
             h->launches.back().n = 0;
+
             h->launches.back().chunks = 0;
         }
         Table<LARGE>& t = h->launches.back();
@@ -494,7 +606,13 @@ int create(WbBackend* b, const WbAdamTensor* tensors, int n, int state_bits, voi
         t.chunks += static_cast<unsigned int>(chunks_of(h->lens[i]));
         offset += padded(h->lens[i]);
     }
-    for (const auto& t : h->launches) {
+    for (auto& t : h->launches) {
+        t.shift = 0;
+        while ((t.chunks >> t.shift) >= HINTS) t.shift++;
+        for (int i = 0, k = 0; i <= HINTS; ++i) {
+            while (k + 1 < t.n && t.first[k + 1] <= (static_cast<uint64_t>(i) << t.shift)) k++;
+            t.hint[i] = static_cast<uint16_t>(k);
+        }
         // at least one block: the norm of nothing is still written
         const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(t.chunks, 8 * b->sm_count)));
         h->norm_grids.push_back(grid);
@@ -598,6 +716,28 @@ extern "C" int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64
     WB_CHECK_CUDA(dev.status);
     WbProfileScope ps(b, h->bits == 32 ? "adam_multi" : "adam_multi_8bit");
     const AdamK k = wb_adam_constants(t, cfg->lr, cfg->beta1, cfg->beta2, cfg->eps, cfg->weight_decay, cfg->decoupled, grad_scale);
+    AdamK8 k8;
+    auto twice = [](float v) {
+        uint32_t bits;
+        memcpy(&bits, &v, 4);
+        return Pair<float>{static_cast<uint64_t>(bits) << 32 | bits};
+    };
+    k8.b1 = twice(k.b1);
+    k8.omb1 = twice(k.omb1);
+    k8.b2 = twice(k.b2);
+    k8.omb2 = twice(k.omb2);
+    k8.minus_inv_sqrt_bc2 = twice(-k.inv_sqrt_bc2);
+    k8.minus_eps = twice(-k.eps);
+    k8.inv_sqrt_bc2 = k.inv_sqrt_bc2;
+    k8.eps = k.eps;
+    k8.step = k.step_size;
+    k8.eps_normal = k.eps >= 8.6736173798840355e-19f && k.inv_sqrt_bc2 <= 1048576.f;
+    k8.minus_step = twice(-k.step_size);
+    k8.minus_zero = twice(-0.f);
+    k8.gscale = k.scale_grad ? k.gscale : 1.f;
+    k8.decay_mul = k.has_wd && k.decoupled ? k.decay_mul : 1.f;
+    k8.wd = k.wd;
+    k8.l2 = k.has_wd && !k.decoupled;
     const int64_t p = h->padded;
     return per_launch(h, [&](int, const auto& tab) -> int {
         constexpr int N = sizeof(tab.first) / sizeof(tab.first[0]);
@@ -607,8 +747,8 @@ extern "C" int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64
             WB_CHECK_CUDA(wb_launch_pdl(adam_multi32_kernel<N>, dim3(tab.chunks), dim3(THREADS), 0, b->stream, tab, m, m + p, k, device_grad_scale));
         } else {
             float* scales = reinterpret_cast<float*>(h->state + 2 * p);
-            WB_CHECK_CUDA(wb_launch_pdl(adam_multi8_kernel<N>, dim3(tab.chunks), dim3(THREADS), 0, b->stream, tab, reinterpret_cast<uint32_t*>(h->state),
-                                        reinterpret_cast<uint32_t*>(h->state + p), scales, scales + p / BLOCK8, k, device_grad_scale, -0.f));
+            WB_CHECK_CUDA(wb_launch_pdl(k.first ? adam_multi8_kernel<N, true> : adam_multi8_kernel<N, false>, dim3(tab.chunks), dim3(THREADS), 0, b->stream, tab, reinterpret_cast<uint32_t*>(h->state),
+                                        reinterpret_cast<uint32_t*>(h->state + p), scales, scales + p / BLOCK8, k8, device_grad_scale));
         }
         WB_LAUNCH_OK(b);
         return WB_OK;
