@@ -102,19 +102,19 @@ def load_library():
 class DeviceStorage:
     """An owned WbStorage handle; returns its block to the backend's arena when collected."""
 
-    __slots__ = ("handle", "backend", "__weakref__")
+    __slots__ = ("handle", "backend", "ptr", "_length", "__weakref__")
 
     def __init__(self, handle: int, backend: "B200Backend"):
         self.handle = handle
         self.backend = backend
-
-    @property
-    def ptr(self) -> int:
-        return self.backend.lib.wb_storage_data(self.handle)
+        self.ptr = backend.lib.wb_storage_data(handle)  # neither address nor length changes while the handle lives
+        self._length = None
 
     @property
     def length(self) -> int:
-        return self.backend.lib.wb_storage_len(self.handle)
+        if self._length is None:
+            self._length = self.backend.lib.wb_storage_len(self.handle)
+        return self._length
 
     def __del__(self):
         be = self.backend

@@ -129,13 +129,14 @@ def contiguous_strides(shape: Sequence[int]) -> List[int]:
 class Layout:
     """crates/weta-core/src/layout.rs:16-21: shape, strides and offset, all in elements."""
 
-    __slots__ = ("shape", "strides", "offset")
+    __slots__ = ("shape", "strides", "offset", "_view")
 
     def __init__(self, shape: Sequence[int], strides: Sequence[int], offset: int = 0):
         assert len(shape) == len(strides)
         self.shape = tuple(int(s) for s in shape)
         self.strides = tuple(int(s) for s in strides)
         self.offset = int(offset)
+        self._view = None
 
     @staticmethod
     def contiguous(shape: Sequence[int]) -> "Layout":
@@ -216,15 +217,14 @@ class Layout:
         return off.reshape(-1)
 
     def view(self, data: int, dtype: int) -> WbView:
-        assert self.ndim <= MAX_DIMS, f"at most {MAX_DIMS} dims are supported, got shape {self.shape}"
-        v = WbView()
+        form = self._view
+        if form is None:  # what does not depend on the storage; filling the arrays costs ten times a copy of the whole
+            assert self.ndim <= MAX_DIMS, f"at most {MAX_DIMS} dims are supported, got shape {self.shape}"
+            rest = MAX_DIMS - self.ndim
+            form = self._view = WbView(None, 0, self.ndim, self.shape + (1,) * rest, self.strides + (0,) * rest, self.offset)
+        v = WbView.from_buffer_copy(form)
         v.data = data
         v.dtype = dtype
-        v.ndim = self.ndim
-        for i in range(MAX_DIMS):
-            v.shape[i] = self.shape[i] if i < self.ndim else 1
-            v.stride[i] = self.strides[i] if i < self.ndim else 0
-        v.offset = self.offset
         return v
 
     def __repr__(self):

@@ -84,13 +84,13 @@ def layer_norm_bwd(be: B200Backend, x: DeviceStorage, lx: Layout, dy: DeviceStor
     """
     _declare(be.lib)
     vx, vg = lx.view(x.ptr, dt), ldy.view(dy.ptr, dt)
-    valid = 1 <= normalized_dims <= lx.ndim and DType.is_float(dt)
-    rows, cols = _rows_cols(lx, normalized_dims) if valid else (0, 1)
-    if out is None:
-        out = (be.alloc(lx.numel(), dt), be.alloc(cols, dt), be.alloc(cols, dt)) if valid else (None, None, None)
-    dx, dweight, dbias = out
-    if workspace is None and valid and cols and (dweight is not None or dbias is not None):
-        workspace = layer_norm_workspace(be, rows, cols, dt)
+    if (out is None or workspace is None) and 1 <= normalized_dims <= lx.ndim and DType.is_float(dt):  # else: refused below
+        rows, cols = _rows_cols(lx, normalized_dims)
+        if out is None:
+            out = (be.alloc(lx.numel(), dt), be.alloc(cols, dt), be.alloc(cols, dt))
+        if workspace is None and cols and (out[1] is not None or out[2] is not None):
+            workspace = layer_norm_workspace(be, rows, cols, dt)
+    dx, dweight, dbias = out if out is not None else (None, None, None)
     size = 0 if workspace is None else workspace.length * DType.size(dt)
     be.check(be.lib.wb_layer_norm_bwd(be.handle, vx, vg, normalized_dims, _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight),
                                       _ptr(dbias), _ptr(workspace), size))
