@@ -400,15 +400,14 @@ __device__ __forceinline__ void cluster_sum(T (&s)[K], T (*peers)[CL][2], int ra
 
 // Backward.  TPR threads hold a row; narrower rows share a warp.  The weight's and the bias's gradients of a thread's columns
 // stay in its registers over all rows it sees; at the end the threads of a column are joined in shared memory and the block
-// leaves one row of partials.  Rows wider than 512 threads hold are cut over the CTAs of a cluster, which exchange the
-// two sums.
+// leaves one row of partials.
 // How rows lie to 16-byte boundaries.  ALIGNED: every row of x, dy and the result starts and ends on one, so no unit is cut.
 // The others cut units at the rows' ends.  SHIFTED: the three share each row's misalignment and a slot holds one row, between
 // zeros that no copy writes over.  MIXED: they do not share it; x and dy are read from shared memory element by element, and a
 // cut unit's foreign elements are replaced.  ELEMENTS, for rows so short that a span of one row would be all overhead: no
 // units, thread t holds the columns t, t + TPR, ... of rows of any misalignment.
 enum { ALIGNED, SHIFTED, MIXED, ELEMENTS };
-template <class T, int TPR, int NV, int CL, int MODE>
+template <class T, int TPR, int NV, int MODE>
 __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* __restrict__ x, const T* __restrict__ dy,
                                                                                           const SpanShape sh, const T* __restrict__ w,
                                                                                           const T* __restrict__ mean, const T* __restrict__ rstd,
@@ -418,24 +417,19 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
     constexpr int N = SPAN_THREADS, GT = TPR < 32 ? 32 : TPR, G = N / GT, SUBS = GT / TPR, U = UNIT<T>, H = U / 2, E = NV * U, LINES = N / TPR;
     constexpr bool HALVES = TPR >= 256;
     static_assert(MODE != ELEMENTS || TPR <= 32, "short rows");
-    static_assert(CL == 1 || LINES == 1, "a cluster's row takes the whole block");
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ T part[G][TPR > 32 ? 4 * TPR / 32 : 1];
-    __shared__ T peers[CL > 1 ? 2 : 1][CL][2];
     __shared__ uint64_t full[G][MOST_RING];
     __shared__ int line_mis[LINES];
     wb_pdl_enter();
     const int group = threadIdx.x / GT, g = threadIdx.x % GT, sub = g / TPR;
-    const int rank = CL > 1 ? static_cast<int>(blockIdx.x) % CL : 0;
-    const int slab = static_cast<int>(blockIdx.x) / CL, slabs = static_cast<int>(gridDim.x) / CL;
+    const int slab = static_cast<int>(blockIdx.x), slabs = static_cast<int>(gridDim.x);
     const int groups = slabs * G, first = slab * G + group;
     Columns<T, TPR, NV> col;
     col.t = g % TPR;
-    col.u0 = rank * sh.units;
+    col.u0 = 0;
     col.mis = MODE == ELEMENTS ? 0 : misalignment(ref + (static_cast<int64_t>(first) * sh.r + sub) * sh.pitch_ref);
-    const int from = CL > 1 ? max(0, col.u0 * U - col.mis) : 0;  // this CTA's columns [from, to)
-    const int to = CL > 1 ? min(sh.cols, (col.u0 + sh.units) * U - col.mis) : sh.cols;
-    col.cols = to;
+    col.cols = sh.cols;
     const bool whole = col.all_whole();
     auto column = [&](int j, int e) { return MODE == ELEMENTS ? (j * U + e) * TPR + col.t : col.first(j) + e; };
     // ring slot: a unit of room, x, a unit of room, dy, mean [32], rstd [32]
@@ -444,11 +438,10 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
     if (g < sh.ring) bar_init(&full[group][g]);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncthreads();
-    if constexpr (CL > 1) cluster_sync();
     if constexpr (MODE == SHIFTED) {  // the ends of each buffer: a unit before and after the first, all from the last on
         for (int k = 0; k < 2 * sh.ring && g < 32; ++k) {
             T* buf = ring + k / 2 * slot_elems + k % 2 * sh.cap;
-            const int e = g < 2 * U ? g - U : max(U, to - from - U) + g - 2 * U;
+            const int e = g < 2 * U ? g - U : max(U, sh.cols - U) + g - 2 * U;
             if (e < sh.cap - U) buf[e] = 0;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -461,7 +454,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
 #pragma unroll
         for (int i = 0; i < H; ++i) {
             const int c = column(j, 2 * i), d = column(j, 2 * i + 1);
-            const bool a = c >= from && c < to, b = d >= from && d < to;
+            const bool a = c >= 0 && c < sh.cols, b = d >= 0 && d < sh.cols;
             wv[j][i] = pair(a ? (w ? w[c] : T(1)) : T(0), b ? (w ? w[d] : T(1)) : T(0));
             aw[j][i] = ab[j][i] = pair(T(0), T(0));
         }
@@ -472,10 +465,10 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
         if (span < sh.spans) {
             const int64_t row0 = static_cast<int64_t>(span) * sh.r;
             const int nr = static_cast<int>(min(static_cast<int64_t>(sh.r), sh.rows - row0));
-            const int n = sh.r > 1 ? nr * sh.cols : to - from;
+            const int n = nr * sh.cols;
             T* base = ring + slot * slot_elems;
-            const T* px = x + row0 * sh.pitch_x + from;
-            const T* pg = dy + row0 * sh.pitch_g + from;
+            const T* px = x + row0 * sh.pitch_x;
+            const T* pg = dy + row0 * sh.pitch_g;
             if (g == 0) {
                 const Split<T> sx(px, n), sg(pg, n);
                 if (part != 2) {
@@ -517,11 +510,11 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
         const int nr = static_cast<int>(min(static_cast<int64_t>(sh.r), sh.rows - row0));
         const T* base = ring + slot * slot_elems;
         // unit j of row r starts at base[off + r cols + (j TPR + t) U]
-        const int shift = MODE == ELEMENTS ? 0 : col.u0 * U - col.mis - from + col.t * U;
+        const int shift = MODE == ELEMENTS ? 0 : col.t * U - col.mis;
         const T *span_x = base + shift, *span_g = base + sh.cap + shift;
         if (MODE != ALIGNED) {
-            span_x += misalignment(x + row0 * sh.pitch_x + from);
-            span_g += misalignment(dy + row0 * sh.pitch_g + from);
+            span_x += misalignment(x + row0 * sh.pitch_x);
+            span_g += misalignment(dy + row0 * sh.pitch_g);
         }
         for (int r0 = 0; r0 < nr; r0 += SUBS) {  // the same number of turns for every lane of a warp
             const bool live = SUBS == 1 || r0 + sub < nr;
@@ -537,19 +530,19 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
                     if constexpr (MODE == ELEMENTS) {
 #pragma unroll
                         for (int i = 0; i < H; ++i) {  // behind the row's end: its last element, which has no weight there
-                            const int c = min(column(j, 2 * i), to - 1), d = min(column(j, 2 * i + 1), to - 1);
+                            const int c = min(column(j, 2 * i), sh.cols - 1), d = min(column(j, 2 * i + 1), sh.cols - 1);
                             xh[j][i] = pair(bx[c], bx[d]);
                             up[i] = pair(bg[c], bg[d]);
                         }
                     } else {
                         // a unit behind the row's end (of the last vector only, in a row of its own): any that is there
-                        const int at = (CL == 1 && j < NV - 1) || col.some(j) ? j * TPR * U : -col.t * U;
+                        const int at = j < NV - 1 || col.some(j) ? j * TPR * U : -col.t * U;
                         load_unit<T, MODE != MIXED>(bx + at, xh[j]);
                         load_unit<T, MODE != MIXED>(bg + at, up);
                     }
                     if constexpr (decltype(edges)::value) {  // what is not of this row counts as a mean value without gradient
-                        replace_outside(col.first(j), to, mu, xh[j]);
-                        replace_outside(col.first(j), to, T(0), up);
+                        replace_outside(col.first(j), sh.cols, mu, xh[j]);
+                        replace_outside(col.first(j), sh.cols, T(0), up);
                     }
 #pragma unroll
                     for (int i = 0; i < H; ++i) {
@@ -574,7 +567,6 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
             s[1] = lo + hi;
             if constexpr (TPR > 32) settle(sh.ring - 2);
             row_sum<T, TPR, G, 2>(s, part[group], 1 + group, turn, [&]() { fetch(span + sh.ring * groups, slot, HALVES ? 1 : 0); });
-            if constexpr (CL > 1) cluster_sum<T, CL, 2>(s, peers, rank, turn);
             const T k0 = -rs * (s[0] * inv_cols), k1 = -rs * (s[1] * inv_cols);
             const Pair<T> k0p = pair(k0, k0), k1p = pair(k1, k1);
             if (live) {
@@ -589,11 +581,11 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
                         for (int i = 0; i < H; ++i) {
                             T a, b;
                             unpair(o[i], a, b);
-                            if (column(j, 2 * i) < to) dr[column(j, 2 * i)] = a;
-                            if (column(j, 2 * i + 1) < to) dr[column(j, 2 * i + 1)] = b;
+                            if (column(j, 2 * i) < sh.cols) dr[column(j, 2 * i)] = a;
+                            if (column(j, 2 * i + 1) < sh.cols) dr[column(j, 2 * i + 1)] = b;
                         }
-                    } else if (MODE == ALIGNED ? (CL == 1 && j < NV - 1) || col.some(j) : whole || col.whole(j)) store_unit(dr + col.first(j), o);
-                    else if (MODE != ALIGNED) store_part(dr, col.first(j), to, o);
+                    } else if (MODE == ALIGNED ? j < NV - 1 || col.some(j) : whole || col.whole(j)) store_unit(dr + col.first(j), o);
+                    else if (MODE != ALIGNED) store_part(dr, col.first(j), sh.cols, o);
                 }
             }
         }
@@ -631,10 +623,10 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
         }
     }
     __syncthreads();
-    for (int c = from + static_cast<int>(threadIdx.x); c < to; c += N) {
+    for (int c = threadIdx.x; c < sh.cols; c += N) {
         T sw = 0, sb = 0;
         for (int k = 0; k < LINES; ++k) {
-            const T* a = joined + k * TPR * E + c + line_mis[k] - col.u0 * U;
+            const T* a = joined + k * TPR * E + c + line_mis[k];
             sw += a[0];
             sb += a[LINES * TPR * E];
         }
@@ -646,6 +638,195 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
             parts[static_cast<int64_t>(slabs + slab) * sh.cols + c] = sb;
         }
     }
+}
+
+// Backward of rows wider than 512 threads hold: a cluster of CTAs takes the row, each its slice of the columns, and they
+// exchange the two sums.  A row goes through two passes over its slot, the first for the sums and the columns' gradients, the
+// second for dx; the cluster's barrier for one row is waited for only after the next row's first pass, which hides it.
+template <class T, int CL, int MODE>
+__global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* __restrict__ x, const T* __restrict__ dy, const SpanShape sh,
+                                                                     const T* __restrict__ w, const T* __restrict__ mean,
+                                                                     const T* __restrict__ rstd, T inv_cols, const T* ref, T* __restrict__ dx,
+                                                                     T* __restrict__ parts, T* __restrict__ dw, T* __restrict__ db) {
+    constexpr int TPR = SPAN_THREADS, NV = 4, U = UNIT<T>, H = U / 2;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    __shared__ T part[4 * TPR / 32];
+    __shared__ T peers[2][CL][2];
+    __shared__ uint64_t full[MOST_RING];
+    wb_pdl_enter();
+    const int t = threadIdx.x, rank = static_cast<int>(blockIdx.x) % CL, slab = static_cast<int>(blockIdx.x) / CL, slabs = static_cast<int>(gridDim.x) / CL;
+    Columns<T, TPR, NV> col;
+    col.t = t;
+    col.u0 = rank * sh.units;
+    col.mis = misalignment(ref + slab * sh.pitch_ref);
+    const int from = max(0, col.u0 * U - col.mis), to = min(sh.cols, (col.u0 + sh.units) * U - col.mis);  // this CTA's columns
+    col.cols = to;
+    const bool whole = col.all_whole();
+    const int slot_elems = 2 * sh.cap + 64;  // see ln_bwd_span_kernel
+    T* ring = reinterpret_cast<T*>(smem_raw) + U;
+    if (t < sh.ring) bar_init(&full[t]);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    if constexpr (MODE == SHIFTED) {
+        for (int k = 0; k < 2 * sh.ring && t < 32; ++k) {
+            T* buf = ring + k / 2 * slot_elems + k % 2 * sh.cap;
+            const int e = t < 2 * U ? t - U : max(U, to - from - U) + t - 2 * U;
+            if (e < sh.cap - U) buf[e] = 0;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+    }
+    Pair<T> wv[NV][H], aw[NV][H], ab[NV][H];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const int c = col.first(j) + 2 * i;
+            const bool a = c >= from && c < to, b = c + 1 >= from && c + 1 < to;
+            wv[j][i] = pair(a ? (w ? w[c] : T(1)) : T(0), b ? (w ? w[c + 1] : T(1)) : T(0));
+            aw[j][i] = ab[j][i] = pair(T(0), T(0));
+        }
+    auto fetch = [&](int row, int slot) {
+        if (t >= 32) return;
+        if (row < sh.spans) {
+            T* base = ring + slot * slot_elems;
+            const T* px = x + row * sh.pitch_x + from;
+            const T* pg = dy + row * sh.pitch_g + from;
+            if (t == 0) {
+                const Split<T> sx(px, to - from), sg(pg, to - from);
+                bar_expect(&full[slot], static_cast<uint32_t>((sx.mid + sg.mid) * sizeof(T)));
+                fetch_units(base, px, sx, &full[slot]);
+                fetch_units(base + sh.cap, pg, sg, &full[slot]);
+                copy_one(base + 2 * sh.cap - U, mean + row);
+                copy_one(base + 2 * sh.cap - U + 32, rstd + row);
+            }
+            if (MODE != ALIGNED && t < 16) fetch_ends(base + (t < 8 ? 0 : sh.cap), t < 8 ? px : pg, to - from, t & 7);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // xhat and dy of unit j of a row in a slot
+    auto load = [&](int row, int slot, int j, T mu, const Pair<T>& minus_mu, const Pair<T>& rs2, Pair<T>(&xh)[H], Pair<T>(&up)[H]) {
+        const T* base = ring + slot * slot_elems + col.u0 * U - col.mis - from + t * U + (col.some(j) ? j * TPR * U : -t * U);
+        int mx = 0, mg = 0;
+        if (MODE != ALIGNED) {
+            mx = misalignment(x + row * sh.pitch_x + from);
+            mg = misalignment(dy + row * sh.pitch_g + from);
+        }
+        load_unit<T, MODE != MIXED>(base + mx, xh);
+        load_unit<T, MODE != MIXED>(base + sh.cap + mg, up);
+        if (MODE == MIXED && !whole) {
+            replace_outside(col.first(j), to, mu, xh);
+            replace_outside(col.first(j), to, T(0), up);
+        }
+#pragma unroll
+        for (int i = 0; i < H; ++i) xh[i] = (xh[i] + minus_mu) * rs2;
+    };
+    for (int k = 0; k < sh.ring; ++k) fetch(slab + k * slabs, k);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+
+    unsigned int turn = 0;
+    uint32_t limit = POLLS, phase = 0;
+    int slot = 0, before = -1;  // before: the slot of the row whose second pass is due
+    for (int row = slab;; row += slabs) {
+        const bool more = row < sh.spans;
+        T s[2] = {0, 0};
+        if (more) {
+            bar_wait(&full[slot], phase, limit);
+            const T mu = ring[slot * slot_elems + 2 * sh.cap - U], rs = ring[slot * slot_elems + 2 * sh.cap - U + 32];
+            const Pair<T> minus_mu = pair(-mu, -mu), rs2 = pair(rs, rs);
+            Pair<T> s0 = pair(T(0), T(0)), s1 = s0;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                Pair<T> xh[H], up[H];
+                load(row, slot, j, mu, minus_mu, rs2, xh, up);
+#pragma unroll
+                for (int i = 0; i < H; ++i) {
+                    const Pair<T> gv = up[i] * wv[j][i];
+                    aw[j][i] = muladd(up[i], xh[i], aw[j][i]);
+                    ab[j][i] = ab[j][i] + up[i];
+                    s0 = s0 + gv;
+                    s1 = muladd(gv, xh[i], s1);
+                }
+            }
+            T lo, hi;
+            unpair(s0, lo, hi);
+            s[0] = lo + hi;
+            unpair(s1, lo, hi);
+            s[1] = lo + hi;
+            if (dx) row_sum<T, TPR, 1, 2>(s, part, 1, turn);
+        }
+        if (dx) {
+            T total[2] = {0, 0};
+            if (before >= 0) {  // the sums of the row before have arrived: written before the barrier that every thread waits for
+                asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+#pragma unroll
+                for (int q = 0; q < CL; ++q) {
+                    total[0] += peers[(turn - (more ? 1 : 0)) & 1][q][0];
+                    total[1] += peers[(turn - (more ? 1 : 0)) & 1][q][1];
+                }
+            }
+            if (more) {
+                if (t < CL) {
+                    uint32_t remote;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(peers[turn & 1][rank])), "r"(t));
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        if constexpr (sizeof(T) == 4) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote + 4 * k), "f"(s[k]) : "memory");
+                        else asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote + 8 * k), "d"(s[k]) : "memory");
+                    }
+                }
+                __syncwarp();
+                asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+            }
+            if (before >= 0) {
+                const int old = row - slabs;
+                const T mu = ring[before * slot_elems + 2 * sh.cap - U], rs = ring[before * slot_elems + 2 * sh.cap - U + 32];
+                const Pair<T> minus_mu = pair(-mu, -mu), rs2 = pair(rs, rs);
+                const T k0 = -rs * (total[0] * inv_cols), k1 = -rs * (total[1] * inv_cols);
+                const Pair<T> k0p = pair(k0, k0), k1p = pair(k1, k1);
+                T* dr = dx + static_cast<int64_t>(old) * sh.cols;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    Pair<T> xh[H], up[H], o[H];
+                    load(old, before, j, mu, minus_mu, rs2, xh, up);
+#pragma unroll
+                    for (int i = 0; i < H; ++i) o[i] = muladd(up[i] * wv[j][i], rs2, muladd(xh[i], k1p, k0p));
+                    if (whole || col.whole(j)) store_unit(dr + col.first(j), o);
+                    else if (MODE != ALIGNED) store_part(dr, col.first(j), to, o);
+                }
+            }
+        }
+        if (!more) break;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");  // the next row's small copies, one turn old
+        __syncthreads();                                      // ... known to all, and the slot behind is read
+        const int done = dx ? before : slot;
+        if (done >= 0) fetch(dx ? row + (sh.ring - 1) * slabs : row + sh.ring * slabs, done);
+        before = slot;
+        slot = slot == sh.ring - 1 ? 0 : slot + 1;
+        phase ^= slot == 0;
+    }
+    if (!parts) return;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int c = col.first(j) + i;
+            if (c < from || c >= to) continue;
+            T a, b;
+            unpair(aw[j][i / 2], a, b);
+            const T sw = i % 2 ? b : a;
+            unpair(ab[j][i / 2], a, b);
+            const T sb = i % 2 ? b : a;
+            if (slabs == 1) {
+                if (dw) dw[c] = sw;
+                if (db) db[c] = sb;
+            } else {
+                parts[static_cast<int64_t>(slab) * sh.cols + c] = sw;
+                parts[static_cast<int64_t>(slabs + slab) * sh.cols + c] = sb;
+            }
+        }
 }
 
 // Forward of wide rows, through the ring: a block's 512 threads, or those of a cluster, hold the row in registers from its one
@@ -1083,7 +1264,7 @@ int ring_depth(size_t slots, int cl) {
     return std::max(2, std::min({fit, MOST_RING, cl > 1 ? 3 : static_cast<int>(((128 << 10) + slots / 2) / slots)}));
 }
 
-// Threads per row, units per thread and CTAs per row for rows of up to `units` units: the fewest threads that hold the row.
+// Threads per row and units per thread for rows of up to `units` units: the fewest threads that hold the row.
 // Rows that share a warp have to lie end to end and uncut (`shared`).
 template <class F>
 bool choose_span(int64_t units, bool shared, F&& f) {
@@ -1094,22 +1275,15 @@ bool choose_span(int64_t units, bool shared, F&& f) {
         const int nv = static_cast<int>((units + TPR - 1) / TPR);
         using One = std::integral_constant<int, 1>;
         if constexpr (TPR == 8 || TPR == 32) {
-            if (nv <= 1) return f(tpr, One{}, One{}), true;
-            if (nv <= 2) return f(tpr, std::integral_constant<int, 2>{}, One{}), true;
+            if (nv <= 1) return f(tpr, One{}), true;
+            if (nv <= 2) return f(tpr, std::integral_constant<int, 2>{}), true;
         }
-        if (nv <= 3) return f(tpr, std::integral_constant<int, 3>{}, One{}), true;
-        return f(tpr, std::integral_constant<int, 4>{}, One{}), true;
+        if (nv <= 3) return f(tpr, std::integral_constant<int, 3>{}), true;
+        return f(tpr, std::integral_constant<int, 4>{}), true;
     };
-    if (per(std::integral_constant<int, 8>{}) || per(std::integral_constant<int, 16>{}) || per(std::integral_constant<int, 32>{}) ||
-        per(std::integral_constant<int, 64>{}) || per(std::integral_constant<int, 128>{}) || per(std::integral_constant<int, 256>{}) ||
-        per(std::integral_constant<int, 512>{}))
-        return true;
-    using W = std::integral_constant<int, 512>;
-    using A = std::integral_constant<int, MOST>;
-    if (units <= 2 * 512 * MOST) return f(W{}, A{}, std::integral_constant<int, 2>{}), true;
-    if (units <= 4 * 512 * MOST) return f(W{}, A{}, std::integral_constant<int, 4>{}), true;
-    if (units <= 8 * 512 * MOST) return f(W{}, A{}, std::integral_constant<int, 8>{}), true;
-    return false;
+    return per(std::integral_constant<int, 8>{}) || per(std::integral_constant<int, 16>{}) || per(std::integral_constant<int, 32>{}) ||
+           per(std::integral_constant<int, 64>{}) || per(std::integral_constant<int, 128>{}) || per(std::integral_constant<int, 256>{}) ||
+           per(std::integral_constant<int, 512>{});
 }
 
 template <class T>
@@ -1123,51 +1297,71 @@ bool bwd_spans(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t p
     const bool aligned = per == 1 && reinterpret_cast<uintptr_t>(ref) % 16 == 0;
     const int64_t units = (s.cols + UNIT<T> - 1 + (aligned ? 0 : UNIT<T> - 1)) / UNIT<T>;
     const bool cut = !aligned || s.cols % UNIT<T> != 0;
-    auto go = [&](auto tpr, auto nv, auto cl, auto mode) {
-        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, CL = decltype(cl)::value, MODE = decltype(mode)::value;
+    SpanShape sh;
+    sh.rows = s.rows;
+    sh.cols = static_cast<int>(s.cols);
+    sh.pitch_x = pitch_x;
+    sh.pitch_g = pitch_g;
+    sh.pitch_ref = pitch_ref;
+    const T inv_cols = static_cast<T>(1.0 / static_cast<double>(s.cols));
+    // a slot's buffer behind a unit of room: the misalignment, the run, what a last unit reads behind it
+    auto buffer = [](int64_t run) { return static_cast<int>((run + UNIT<T> - 1) / UNIT<T> * UNIT<T> + 3 * UNIT<T>); };
+    auto go = [&](auto tpr, auto nv, auto mode) {
+        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, MODE = decltype(mode)::value;
         constexpr int N = SPAN_THREADS, GT = TPR < 32 ? 32 : TPR, G = N / GT, SUBS = GT / TPR;
-        SpanShape sh;
-        sh.rows = s.rows;
-        sh.cols = static_cast<int>(s.cols);
-        sh.pitch_x = pitch_x;
-        sh.pitch_g = pitch_g;
-        sh.pitch_ref = pitch_ref;
-        sh.units = static_cast<int>((units + CL - 1) / CL);
+        sh.units = static_cast<int>(units);
         sh.r = GT == 32 && dense && (MODE == ALIGNED || MODE == ELEMENTS) ? rows_per_span<T>(b, s, G, SUBS) : 1;
         sh.spans = static_cast<int>((s.rows + sh.r - 1) / sh.r);
-        // behind a unit of room: the misalignment, the rows, what a last unit reads behind them
-        const int64_t run = CL > 1 ? static_cast<int64_t>(sh.units) * UNIT<T> : sh.r * s.cols;
-        sh.cap = static_cast<int>((run + UNIT<T> - 1) / UNIT<T> * UNIT<T> + 3 * UNIT<T>);
+        sh.cap = buffer(sh.r * s.cols);
         const size_t slots = sizeof(T) * static_cast<size_t>(G) * (2 * sh.cap + 64), join = sizeof(T) * 2 * N * NV * UNIT<T>;
-        sh.ring = ring_depth(slots, CL);
+        sh.ring = ring_depth(slots, 1);
         // one slab saves the launch that joins the partials, about what two more rows in a row take
-        *err = launch_spans<ln_bwd_span_kernel<T, TPR, NV, CL, MODE>, CL>(b, sh, G, std::max(slots * sh.ring, join), MODE == ELEMENTS ? 1 : per, parts ? 3 : 0,
-                                                                         slabs, x, dy, sh, w, mean, rstd,
-                                                                         static_cast<T>(1.0 / static_cast<double>(s.cols)), ref, dx, parts, dw, db);
+        *err = launch_spans<ln_bwd_span_kernel<T, TPR, NV, MODE>, 1>(b, sh, G, std::max(slots * sh.ring, join), MODE == ELEMENTS ? 1 : per, parts ? 3 : 0,
+                                                                    slabs, x, dy, sh, w, mean, rstd, inv_cols, ref, dx, parts, dw, db);
+    };
+    auto go_wide = [&](auto cl, auto mode) {
+        constexpr int CL = decltype(cl)::value, MODE = decltype(mode)::value;
+        sh.units = static_cast<int>((units + CL - 1) / CL);
+        sh.r = 1;
+        sh.spans = static_cast<int>(s.rows);
+        sh.cap = buffer(static_cast<int64_t>(sh.units) * UNIT<T>);
+        const size_t slots = sizeof(T) * (2 * sh.cap + 64);
+        sh.ring = 3;
+        *err = launch_spans<ln_bwd_wide_kernel<T, CL, MODE>, CL>(b, sh, 1, slots * sh.ring, per, parts ? 2 : 0, slabs, x, dy, sh, w, mean, rstd, inv_cols,
+                                                                ref, dx, parts, dw, db);
+        return true;
     };
     if ((cut || !same) && s.cols <= 16 * 4 * UNIT<T>) {
         const int nv = static_cast<int>((s.cols + (s.cols <= 8 * 4 * UNIT<T> ? 8 : 16) * UNIT<T> - 1) / ((s.cols <= 8 * 4 * UNIT<T> ? 8 : 16) * UNIT<T>));
         using M = std::integral_constant<int, ELEMENTS>;
-        using One = std::integral_constant<int, 1>;
-        using N1 = One;
+        using N1 = std::integral_constant<int, 1>;
         using N2 = std::integral_constant<int, 2>;
         using N3 = std::integral_constant<int, 3>;
         using N4 = std::integral_constant<int, 4>;
         using T8 = std::integral_constant<int, 8>;
         using T16 = std::integral_constant<int, 16>;
         if (s.cols <= 8 * 4 * UNIT<T>)
-            nv == 1 ? go(T8{}, N1{}, One{}, M{}) : nv == 2 ? go(T8{}, N2{}, One{}, M{}) : nv == 3 ? go(T8{}, N3{}, One{}, M{}) : go(T8{}, N4{}, One{}, M{});
+            nv == 1 ? go(T8{}, N1{}, M{}) : nv == 2 ? go(T8{}, N2{}, M{}) : nv == 3 ? go(T8{}, N3{}, M{}) : go(T8{}, N4{}, M{});
         else
-            nv == 3 ? go(T16{}, N3{}, One{}, M{}) : go(T16{}, N4{}, One{}, M{});
+            nv == 3 ? go(T16{}, N3{}, M{}) : go(T16{}, N4{}, M{});
         return true;
     }
-    return choose_span(units, dense && !cut && same, [&](auto tpr, auto nv, auto cl) {
+    const bool done = choose_span(units, dense && !cut && same, [&](auto tpr, auto nv) {
         if constexpr (decltype(tpr)::value >= 32) {
-            if (!same) return go(tpr, nv, cl, std::integral_constant<int, MIXED>{});
-            if (cut) return go(tpr, nv, cl, std::integral_constant<int, SHIFTED>{});
+            if (!same) return go(tpr, nv, std::integral_constant<int, MIXED>{});
+            if (cut) return go(tpr, nv, std::integral_constant<int, SHIFTED>{});
         }
-        go(tpr, nv, cl, std::integral_constant<int, ALIGNED>{});
+        go(tpr, nv, std::integral_constant<int, ALIGNED>{});
     });
+    if (done) return true;
+    auto wide = [&](auto mode) {
+        if (units <= 2 * 2048) return go_wide(std::integral_constant<int, 2>{}, mode);
+        if (units <= 4 * 2048) return go_wide(std::integral_constant<int, 4>{}, mode);
+        if (units <= 8 * 2048) return go_wide(std::integral_constant<int, 8>{}, mode);
+        return false;
+    };
+    if (!same) return wide(std::integral_constant<int, MIXED>{});
+    return cut ? wide(std::integral_constant<int, SHIFTED>{}) : wide(std::integral_constant<int, ALIGNED>{});
 }
 
 template <class T>
