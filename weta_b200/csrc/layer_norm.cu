@@ -808,25 +808,19 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
         phase ^= slot == 0;
     }
     if (!parts) return;
+    T* to_w = slabs == 1 ? dw : parts + static_cast<int64_t>(slab) * sh.cols;
+    T* to_b = slabs == 1 ? db : parts + static_cast<int64_t>(slabs + slab) * sh.cols;
+    const bool units = MODE == ALIGNED && ((reinterpret_cast<uintptr_t>(to_w) | reinterpret_cast<uintptr_t>(to_b)) & 15) == 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int c = col.first(j) + i;
-            if (c < from || c >= to) continue;
-            T a, b;
-            unpair(aw[j][i / 2], a, b);
-            const T sw = i % 2 ? b : a;
-            unpair(ab[j][i / 2], a, b);
-            const T sb = i % 2 ? b : a;
-            if (slabs == 1) {
-                if (dw) dw[c] = sw;
-                if (db) db[c] = sb;
-            } else {
-                parts[static_cast<int64_t>(slab) * sh.cols + c] = sw;
-                parts[static_cast<int64_t>(slabs + slab) * sh.cols + c] = sb;
-            }
+    for (int j = 0; j < NV; ++j) {
+        if (units && col.whole(j)) {
+            if (to_w) store_unit(to_w + col.first(j), aw[j]);
+            if (to_b) store_unit(to_b + col.first(j), ab[j]);
+        } else {
+            if (to_w) store_part(to_w, col.first(j), to, aw[j]);
+            if (to_b) store_part(to_b, col.first(j), to, ab[j]);
         }
+    }
 }
 
 // Forward of wide rows, through the ring: a block's 512 threads, or those of a cluster, hold the row in registers from its one
@@ -988,14 +982,13 @@ __global__ void __launch_bounds__(THREADS) ln_dw_any_kernel(const T* __restrict_
     }
 }
 
-// Sums the slabs of both partial arrays: 32 columns per block, 32 lines of threads that take every 32nd slab, joined in
-// order.  A line's loads (ten for 296 slabs) are all in flight at once: with eight lines and their loads in turn this
-// kernel took 10 us whatever the size.
-constexpr int JOIN_LINES = 32;
-template <class T>
-__global__ void __launch_bounds__(32 * JOIN_LINES) ln_dw_join_kernel(const T* __restrict__ parts, int slabs, int64_t cols, T* __restrict__ dw,
-                                                                     T* __restrict__ db) {
-    __shared__ double sum[JOIN_LINES][33];
+// Sums the slabs of both partial arrays: 32 columns per block, LINES lines of threads that take every LINES-th slab, joined in
+// order.  A line's loads are all in flight at once (ten: 32 lines reach 320 slabs, eight 80, four 40); 296 slabs by eight lines, their loads
+// in turn, took 10 us whatever the size, and 8 slabs of 16384 columns by 32 lines as long.
+template <class T, int LINES>
+__global__ void __launch_bounds__(32 * LINES) ln_dw_join_kernel(const T* __restrict__ parts, int slabs, int64_t cols, T* __restrict__ dw,
+                                                                T* __restrict__ db) {
+    __shared__ double sum[LINES][33];
     wb_pdl_enter();
     T* out = blockIdx.y == 0 ? dw : db;
     if (!out) return;
@@ -1005,11 +998,11 @@ __global__ void __launch_bounds__(32 * JOIN_LINES) ln_dw_join_kernel(const T* __
     if (c < cols) {
         const T* p = parts + static_cast<int64_t>(blockIdx.y) * slabs * cols + c;
         constexpr int BATCH = 10;
-        for (int k0 = line; k0 < slabs; k0 += JOIN_LINES * BATCH) {
+        for (int k0 = line; k0 < slabs; k0 += LINES * BATCH) {
             T v[BATCH];
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
-                const int k = k0 + j * JOIN_LINES;
+                const int k = k0 + j * LINES;
                 v[j] = k < slabs ? p[static_cast<int64_t>(k) * cols] : T(0);
             }
 #pragma unroll
@@ -1018,12 +1011,17 @@ __global__ void __launch_bounds__(32 * JOIN_LINES) ln_dw_join_kernel(const T* __
     }
     sum[line][lane] = acc;
     __syncthreads();
-    // transposed: a warp joins one column
-    acc = sum[lane][line];
+    if constexpr (LINES == 32) {  // transposed: a warp joins one column
+        acc = sum[lane][line];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
-    const int64_t to = static_cast<int64_t>(blockIdx.x) * 32 + line;
-    if (lane == 0 && to < cols) out[to] = static_cast<T>(acc);
+        for (int d = 16; d > 0; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
+        const int64_t to = static_cast<int64_t>(blockIdx.x) * 32 + line;
+        if (lane == 0 && to < cols) out[to] = static_cast<T>(acc);
+    } else if (line == 0 && c < cols) {
+#pragma unroll
+        for (int k = 1; k < LINES; ++k) acc += sum[k][lane];
+        out[c] = static_cast<T>(acc);
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
@@ -1471,8 +1469,11 @@ int bwd_typed(WbBackend* b, const WbView* x, const WbView* dy, int nd, const Sha
                                     parts, slabs));
         WB_LAUNCH_OK(b);
     }
-    WB_CHECK_CUDA(wb_launch_pdl(ln_dw_join_kernel<T>, dim3(static_cast<unsigned>((s.cols + 31) / 32), 2), dim3(32 * JOIN_LINES), 0, b->stream,
-                                static_cast<const T*>(parts), slabs, s.cols, dw, db));
+    const dim3 strips(static_cast<unsigned>((s.cols + 31) / 32), 2);
+    const T* joined = parts;
+    if (slabs <= 40) WB_CHECK_CUDA(wb_launch_pdl(ln_dw_join_kernel<T, 4>, strips, dim3(32 * 4), 0, b->stream, joined, slabs, s.cols, dw, db));
+    else if (slabs <= 80) WB_CHECK_CUDA(wb_launch_pdl(ln_dw_join_kernel<T, 8>, strips, dim3(32 * 8), 0, b->stream, joined, slabs, s.cols, dw, db));
+    else WB_CHECK_CUDA(wb_launch_pdl(ln_dw_join_kernel<T, 32>, strips, dim3(32 * 32), 0, b->stream, joined, slabs, s.cols, dw, db));
     WB_LAUNCH_OK(b);
     return WB_OK;
 }

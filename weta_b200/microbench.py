@@ -11,7 +11,8 @@ f32 N(0,1) from the counter RNG.  Tensors are larger than the 126 MB L2 where th
 the softmax-cross-entropy logits (33 MB) rotate through 8 buffers so each launch reads from HBM.
 Algorithmic bytes: unary 8 B/elem, binary 12 B/elem, mul backward 20 B/elem (read g, a, b; write g*b, g*a: timed
 as the two trait launches the reference issues, which move 24), ReLU backward 12 B/elem (the fused wb_relu_bwd), BN
-fwd 12 / bwd 20 B/elem, softmax-CE fused fwd+bwd 8*N*C, dropout mask 4 B/elem, Adam 28 B/elem; contractions 2*M*N*K flop.
+fwd 12 / bwd 20 B/elem, softmax-CE fused fwd+bwd 8*N*C, dropout mask 4 B/elem, Adam 28 B/elem (16 with 8-bit state),
+layer norm fwd 8 / bwd 12 B/elem, gradient norm 4 B/elem; contractions 2*M*N*K flop.
 """
 from __future__ import annotations
 
@@ -22,6 +23,7 @@ import os
 
 import numpy as np
 
+from . import layers, optim
 from .backend import B200Backend, WbConvParams
 from .core import BinaryOp, Distribution, DType, Im2ColParams, Layout, ReduceOp, UnaryOp
 from .trainer import _declare
@@ -194,6 +196,45 @@ def main():
         be.check(lib.wb_adam_step(H, P(th.storage), P(gr.storage), P(m1.storage), P(v1.storage), na, step[0], 1e-3, 0.9, 0.999, 1e-8, 0.0, 0, 1.0))
 
     rec("adam step", timeit(adam, iters=10), 28 * na)
+
+    # layer normalisation, forward and backward, of a short and a long batch
+    for rows, cols in ((8192, 1000),) if args.quick else ((8192, 1000), (16384, 4096)):
+        e, l = rows * cols, Layout.contiguous([rows, cols])
+        sets = []
+        for i in range(max(1, -(-(300 << 20) // (12 * e)))):  # together larger than L2
+            a, g, wl, bl = randn([rows, cols], 30 + i), randn([rows, cols], 60 + i), randn([cols], 4), randn([cols], 5)
+            outs = [be.alloc(nn, DType.F32) for nn in (e, rows, rows, e, cols, cols)]
+            sets.append((a, g, wl, bl, outs, layers.layer_norm_workspace(be, rows, cols, DType.F32)))
+        turn = [0]
+
+        def ln(backward):
+            turn[0] += 1
+            a, g, wl, bl, outs, work = sets[turn[0] % len(sets)]
+            if backward:
+                layers.layer_norm_bwd(be, a.storage, l, g.storage, l, DType.F32, 1, wl.storage, outs[1], outs[2], out=outs[3:], workspace=work)
+            else:
+                layers.layer_norm_fwd(be, a.storage, l, DType.F32, 1, wl.storage, bl.storage, 1e-5, out=outs[:3])
+
+        rec(f"layer norm fwd [{rows},{cols}]", timeit(lambda: ln(False)), 8 * e)
+        rec(f"layer norm bwd [{rows},{cols}]", timeit(lambda: ln(True)), 12 * e)
+        del sets
+    # the many-tensor step: the same elements as above in 128 tensors
+    each = na // 128
+    for bits in (32, 8):
+        params = [be.wrap_pointer(th.storage.ptr + 4 * i * each, each, DType.F32) for i in range(128)]
+        opt = optim.AdamMulti(be, params, bits)
+        opt.set_grads([be.wrap_pointer(gr.storage.ptr + 4 * i * each, each, DType.F32) for i in range(128)])
+        step[0] = 0
+
+        def many():
+            step[0] += 1
+            opt.step(step[0])
+
+        rec(f"adam step, 128 tensors, {bits}-bit state", timeit(many, iters=10), (28 if bits == 32 else 16) * 128 * each)
+        scalars = (be.alloc(1, DType.F32), be.alloc(1, DType.F32))
+        if bits == 32:
+            rec("gradient norm, 128 tensors", timeit(lambda: opt.grad_norm(1.0, out=scalars), iters=10), 4 * 128 * each)
+        opt.close()
 
     # ---- contraction microbenchmark: forward plus both gradients ---------------------------------
     for mode, mname in ((1, "tf32"), (0, "3xtf32")):
