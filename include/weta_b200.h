@@ -398,8 +398,9 @@ typedef struct WbAdamTensor {
 } WbAdamTensor;
 int64_t wb_adam_multi_state_bytes(const int64_t* lens, int n, int state_bits); /* -1: bad arguments */
 /* Tensors may lie anywhere (4-byte aligned) but not overlap; a length may be 0.  keep_state: the memory holds a saved
- * state; else it is zeroed.  The handle belongs to the backend, which has to outlive it; a handle's calls do not
- * overlap each other (one stream, or ordered by the caller). */
+ * state; else it is zeroed.  Not while the stream is being captured.  The handle belongs to the backend, which has to outlive
+ * it; a handle's calls do not overlap each other (one stream, or ordered by the caller), and a captured graph that holds
+ * its calls needs it alive. */
 int wb_adam_multi_create(WbBackend* b, const WbAdamTensor* tensors, int n, int state_bits, void* state, int64_t state_bytes, int keep_state,
                          WbAdamMulti** out);
 int wb_adam_multi_destroy(WbAdamMulti* h);

@@ -292,6 +292,31 @@ def test_8_bits_at_the_edges(gpu):
     assert np.isfinite(np.delete(m, np.s_[1536:2048])).all() and np.isfinite(np.delete(v, np.s_[1536:2048])).all()
 
 
+@pytest.mark.parametrize("eps", [1e-8, 0.0, 1e-30])
+@pytest.mark.parametrize("scale", [1.0, 1e-12, 1e-17, 1e-20, 1e15, 1e18])
+def test_8_bits_across_the_exponent_range(gpu, eps, scale):
+    """Gradients from tiny to huge, eps down to 0: where the step leaves the range of its fast root and quotient it takes
+    sqrt and division themselves, with the same bits."""
+    rng = np.random.default_rng(3)
+    n = 256 * 30 + 9
+    g = (rng.standard_normal(n) * np.exp(2 * rng.standard_normal(n)) * scale).astype(F)
+    th = rng.standard_normal(n).astype(F)
+    store = gpu.from_host(th)
+    opt = optim.AdamMulti(gpu, [store], 8, lr=1e-2, eps=eps)
+    opt.set_grads([gpu.from_host(g)])
+    p = Plain(n, 8)
+    with np.errstate(all="ignore"):
+        for t in (1, 2, 3):
+            opt.step(t)
+            th = p.step(th, g, t, 1e-2, 0.9, 0.999, eps, 0.0, False, False, None)
+            assert same(down(gpu, store, n), th), t
+            (mc, vc, ms, vs), = state_of(gpu, opt, [n], 8)
+            assert same(ms, p.ms) and same(vs, p.vs), t
+            # at 1e18 squares overflow: such a block's scale is NaN, it reads as NaN whatever its codes, which are not defined
+            keep_m, keep_v = (np.repeat(np.isfinite(a), 256) for a in (p.ms, p.vs))
+            assert same(mc[keep_m], p.mc[keep_m]) and same(vc[keep_v], p.vc[keep_v]), t
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_nothing_is_written_between_the_tensors(gpu, bits):
     """Tensors inside one guarded buffer, in another order than in memory."""
@@ -416,6 +441,13 @@ def test_refusals_on_a_live_handle(gpu):
     for limit in (0.0, -1.0, float("nan")):
         with pytest.raises(BackendError, match="above 0"):
             opt.grad_norm(limit)
+    one = gpu.zeros(2, DType.F32)
+    with pytest.raises(BackendError, match="the two outputs are one"):
+        opt.grad_norm(1.0, out=(one, one))
+    with pytest.raises(BackendError, match="the two outputs are one, or not aligned"):
+        opt.grad_norm(1.0, out=(gpu.wrap_pointer(one.ptr + 2, 1, DType.F32), gpu.zeros(1, DType.F32)))
+    with pytest.raises(BackendError, match="scale is not aligned"):
+        opt.step(1, gpu.wrap_pointer(one.ptr + 1, 1, DType.F32))
     with pytest.raises(BackendError, match="overlap"):
         opt.read_state(out=(gpu.wrap_pointer(opt.state.ptr, 1024, DType.F32), None))
     with pytest.raises(BackendError, match="two tensors"):
@@ -426,6 +458,22 @@ def test_refusals_on_a_live_handle(gpu):
         optim.AdamMulti(gpu, [])
     with pytest.raises(BackendError, match="not 16"):
         optim.AdamMulti(gpu, [a], 16)
+
+
+def test_no_handle_is_made_while_the_stream_is_captured(gpu):
+    import torch
+
+    from weta_b200.backend import B200Backend
+
+    st = torch.cuda.Stream()
+    be = B200Backend(0, stream=st.cuda_stream)
+    a, room = be.zeros(700, DType.F32), be.zeros(8 * pad(700) // 4, DType.F32)
+    be.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        with pytest.raises(BackendError, match="being captured"):
+            optim.AdamMulti(be, [a], state=room)
+    del graph
 
 
 @pytest.mark.parametrize("bits", [32, 8])

@@ -96,9 +96,15 @@ def test_columns(gpu, cols, dt):
 
 
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 1024), (2, 64), (7, 96), (33, 1000), (128, 512), (297, 40), (1000, 33), (2500, 256), (4099, 100),
-                                       (70001, 3), (3001, 777), (1201, 2048), (1111, 4100), (601, 9000)])
+                                       (70001, 3), (3001, 777), (1201, 2048), (1111, 4100), (1400, 4096), (700, 8192), (601, 9000), (400, 9001),
+                                       (330, 16388), (20011, 33), (9000, 250), (6007, 130)])
 def test_rows(gpu, rows, cols):
     both_ways(gpu, rows, cols, DType.F32)
+
+
+@pytest.mark.parametrize("rows,cols", [(3000, 65), (2500, 129), (1500, 1000), (801, 2049), (500, 4099), (310, 6000)])
+def test_rows_in_double_precision(gpu, rows, cols):
+    both_ways(gpu, rows, cols, DType.F64)
 
 
 @pytest.mark.parametrize("cols", [6, 256, 1001, 4096, 16384, 33000])
@@ -124,6 +130,17 @@ def test_rows_of_one_value(gpu, cols, dt):
     assert np.array_equal(get(gpu, m, (4,), dt), x[:, 0])
     assert np.allclose(get(gpu, r, (4,), dt), 256.0, rtol=4 * U[dt], atol=0)
     assert np.array_equal(get(gpu, y, (4, cols), dt), np.broadcast_to(b, (4, cols)))
+
+
+@pytest.mark.parametrize("cols", [3, 41, 97, 250, 1001, 3333, 9001, 12000, 20001])
+def test_rows_of_one_integer(gpu, cols):
+    """Sums of equal small integers are exact in any order, so the mean is that integer and y the bias, whatever 1 / cols is."""
+    x = np.repeat(np.array([7.0, 200.0, -3.0], np.float32)[:, None], cols, 1)
+    l = Layout.contiguous([3, cols])
+    b = np.arange(cols).astype(np.float32)
+    y, m, _ = layers.layer_norm_fwd(gpu, gpu.from_host(x.reshape(-1)), l, DType.F32, 1, None, gpu.from_host(b), 1e-12)
+    assert np.array_equal(get(gpu, m, (3,), DType.F32), x[:, 0])
+    assert np.array_equal(get(gpu, y, (3, cols), DType.F32), np.broadcast_to(b, (3, cols)))
 
 
 @pytest.mark.parametrize("cols", [5, 300, 1024, 4096, 9001])
@@ -160,6 +177,12 @@ VIEWS = {  # name: (storage length, Layout, normalised dims)
     "one value per row": (11, Layout([11, 64], [1, 0], 0), 1),
     "broadcast middle": (3 * 32, Layout([3, 4, 32], [32, 0, 1], 0), 1),
     "inner dims that do not merge": (3 * 8 * 16, Layout([3, 16, 8], [128, 1, 16], 0), 2),
+    "slice of short odd rows": (50 * 101 + 9, Layout([50, 100], [101, 1], 1), 1),
+    "slice of wide rows": (7 * 9100, Layout([7, 9001], [9100, 1], 2), 1),
+    "slice of wider odd rows": (3 * 20011 + 5, Layout([3, 20000], [20011, 1], 5), 1),
+    "wide rows back to front": (4 * 12000, Layout([4, 12000], [-12000, 1], 3 * 12000), 1),
+    "a wide row for all": (10004, Layout([9, 10000], [0, 1], 3), 1),
+    "more columns than a cluster holds": (2 * 70000, Layout.contiguous([2, 70000]), 1),
     "eight dims": (2 ** 6 * 9, Layout.contiguous([2, 1, 2, 2, 1, 2, 4, 9]), 3),
 }
 

@@ -14,7 +14,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <new>
+#include <exception>
 
 #include "adam.cuh"
 #include "common.h"
@@ -620,6 +620,9 @@ int create(WbBackend* b, const WbAdamTensor* tensors, int n, int state_bits, voi
     }
     WbDeviceGuard dev(b->ordinal);
     WB_CHECK_CUDA(dev.status);
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    WB_CHECK_CUDA(cudaStreamIsCapturing(b->stream, &capture));
+    WB_REQUIRE(capture == cudaStreamCaptureStatusNone, WB_ERR_INVALID, "wb_adam_multi_create: the stream is being captured; a replay would zero the state");
     WB_TRY(wb_arena_alloc(b, 16 + sizeof(double) * static_cast<size_t>(h->norm_parts), &h->work, &h->work_class));
     WB_CHECK_CUDA(cudaMemsetAsync(h->work, 0, 16, b->stream));
     if (need && !keep_state) WB_CHECK_CUDA(cudaMemsetAsync(state, 0, static_cast<size_t>(need), b->stream));
@@ -644,7 +647,7 @@ extern "C" int wb_adam_multi_create(WbBackend* b, const WbAdamTensor* tensors, i
     try {
         h = new WbAdamMulti();
         status = create(b, tensors, n, state_bits, state, state_bytes, keep_state, h);
-    } catch (const std::bad_alloc&) {
+    } catch (const std::exception&) {
         wb_set_error("wb_adam_multi_create: out of host memory");
         status = WB_ERR_OOM;
     }
@@ -689,6 +692,8 @@ extern "C" int wb_adam_multi_set_grads(WbAdamMulti* h, const float* const* grads
 extern "C" int wb_adam_multi_grad_norm(WbAdamMulti* h, double max_norm, float* norm, float* clip_scale) {
     WB_REQUIRE(h && norm, WB_ERR_INVALID, "wb_adam_multi_grad_norm: null pointer");
     WB_REQUIRE(h->grads_set, WB_ERR_INVALID, "wb_adam_multi_grad_norm: no gradients were set");
+    WB_REQUIRE((reinterpret_cast<uintptr_t>(norm) | reinterpret_cast<uintptr_t>(clip_scale)) % 4 == 0 && norm != clip_scale, WB_ERR_INVALID,
+               "wb_adam_multi_grad_norm: the two outputs are one, or not aligned to 4 bytes");
     WB_REQUIRE(!clip_scale || max_norm > 0.0, WB_ERR_INVALID, "wb_adam_multi_grad_norm: the largest norm has to be above 0, got %g", max_norm);
     WbBackend* b = h->b;
     WbDeviceGuard dev(b->ordinal);
@@ -697,7 +702,7 @@ extern "C" int wb_adam_multi_grad_norm(WbAdamMulti* h, double max_norm, float* n
     unsigned int* counter = static_cast<unsigned int*>(h->work);
     double* parts = reinterpret_cast<double*>(static_cast<char*>(h->work) + 16);
     int at = 0;
-    return per_launch(h, [&](int l, const auto& tab) -> int {
+    const int status = per_launch(h, [&](int l, const auto& tab) -> int {
         constexpr int N = sizeof(tab.first) / sizeof(tab.first[0]);
         WB_CHECK_CUDA(wb_launch_pdl(grad_norm_kernel<N>, dim3(h->norm_grids[l]), dim3(THREADS), 0, b->stream, tab, parts, at, h->norm_parts, counter,
                                     max_norm, norm, clip_scale));
@@ -705,11 +710,14 @@ extern "C" int wb_adam_multi_grad_norm(WbAdamMulti* h, double max_norm, float* n
         at += h->norm_grids[l];
         return WB_OK;
     });
+    if (status != WB_OK) (void)cudaMemsetAsync(counter, 0, sizeof(unsigned int), b->stream);  // some blocks of this call will not arrive
+    return status;
 }
 
 extern "C" int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64_t t, double grad_scale, const float* device_grad_scale) {
     WB_REQUIRE(h && cfg, WB_ERR_INVALID, "wb_adam_multi_step: null pointer");
     WB_REQUIRE(h->grads_set, WB_ERR_INVALID, "wb_adam_multi_step: no gradients were set");
+    WB_REQUIRE(reinterpret_cast<uintptr_t>(device_grad_scale) % 4 == 0, WB_ERR_INVALID, "wb_adam_multi_step: the scale is not aligned to 4 bytes");
     WB_REQUIRE(t >= 1 && t <= INT32_MAX, WB_ERR_INVALID, "wb_adam_multi_step: step counts from 1 to 2^31 - 1");
     WbBackend* b = h->b;
     WbDeviceGuard dev(b->ordinal);

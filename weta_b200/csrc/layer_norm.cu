@@ -157,7 +157,7 @@ constexpr int fwd_threads = TPR < 64 ? 128 : TPR;
 
 template <class T, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* __restrict__ x, int64_t pitch, int64_t rows, int cols,
-                                                                       const T* __restrict__ w, const T* __restrict__ bias, T eps, T inv_cols,
+                                                                       const T* __restrict__ w, const T* __restrict__ bias, T eps,
                                                                        T* __restrict__ y, T* __restrict__ mean_out, T* __restrict__ rstd_out) {
     constexpr int G = fwd_threads<TPR> / TPR;
     __shared__ T part[G][TPR > 32 ? 2 * TPR / 32 : 1];
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* 
     }
     unsigned int turn = 0;
     row_sum<T, TPR, G, 1>(s, part[group], 1 + group, turn);
-    const T mean = s[0] * inv_cols;
+    const T n = static_cast<T>(cols), mean = s[0] / n;  // a division: the mean of equal values is that value where their sum is exact
     T q[1] = {0};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* 
         }
     }
     row_sum<T, TPR, G, 1>(q, part[group], 1 + group, turn);
-    const T rstd = T(1) / sqrt(q[0] * inv_cols + eps);
+    const T rstd = T(1) / sqrt(q[0] / n + eps);
     if (!live) return;
     T* yr = y + row * cols;
 #pragma unroll
@@ -408,12 +408,10 @@ __device__ __forceinline__ void cluster_sum(T (&s)[K], T (*peers)[CL][2], int ra
 // units, thread t holds the columns t, t + TPR, ... of rows of any misalignment.
 enum { ALIGNED, SHIFTED, MIXED, ELEMENTS };
 template <class T, int TPR, int NV, int MODE>
-__global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* __restrict__ x, const T* __restrict__ dy,
-                                                                                          const SpanShape sh, const T* __restrict__ w,
-                                                                                          const T* __restrict__ mean, const T* __restrict__ rstd,
-                                                                                          T inv_cols, const T* ref, T* __restrict__ dx,
-                                                                                          T* __restrict__ parts, T* __restrict__ dw,
-                                                                                          T* __restrict__ db) {
+__global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* __restrict__ x, const T* __restrict__ dy, const SpanShape sh,
+                                                                     const T* __restrict__ w, const T* __restrict__ mean,
+                                                                     const T* __restrict__ rstd, T inv_cols, const T* ref, T* __restrict__ dx,
+                                                                     T* __restrict__ parts, T* __restrict__ dw, T* __restrict__ db) {
     constexpr int N = SPAN_THREADS, GT = TPR < 32 ? 32 : TPR, G = N / GT, SUBS = GT / TPR, U = UNIT<T>, H = U / 2, E = NV * U, LINES = N / TPR;
     constexpr bool HALVES = TPR >= 256;
     static_assert(MODE != ELEMENTS || TPR <= 32, "short rows");
@@ -829,8 +827,8 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
 // [4096, 12000] 98 us against 69 us, [4096, 16384] 115 against 98 us.
 template <class T, int NV, int CL, int MODE>
 __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_fwd_span_kernel(const T* __restrict__ x, const SpanShape sh, const T* __restrict__ w,
-                                                                     const T* __restrict__ bias, T eps, T inv_cols, T* __restrict__ y,
-                                                                     T* __restrict__ mean_out, T* __restrict__ rstd_out) {
+                                                                     const T* __restrict__ bias, T eps, T* __restrict__ y, T* __restrict__ mean_out,
+                                                                     T* __restrict__ rstd_out) {
     constexpr int TPR = SPAN_THREADS, U = UNIT<T>, H = U / 2;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ T part[2 * TPR / 32];
@@ -912,7 +910,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_fwd_span_kernel(const T* _
         settle(sh.ring - 2);
         row_sum<T, TPR, 1, 1>(s, part, 1, turn, [&]() { fetch(row + sh.ring * groups, slot); });
         if constexpr (CL > 1) cluster_sum<T, CL, 1>(s, peers, rank, turn);
-        const T mu = s[0] * inv_cols;
+        const T n = static_cast<T>(sh.cols), mu = s[0] / n;
         const Pair<T> minus_mu = pair(-mu, -mu);
         s2 = pair(T(0), T(0));
 #pragma unroll
@@ -927,7 +925,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_fwd_span_kernel(const T* _
         s[0] = lo + hi;
         row_sum<T, TPR, 1, 1>(s, part, 1, turn);
         if constexpr (CL > 1) cluster_sum<T, CL, 1>(s, peers, rank, turn);
-        const T rs = T(1) / sqrt(s[0] * inv_cols + eps);
+        const T rs = T(1) / sqrt(s[0] / n + eps);
         const Pair<T> rs2 = pair(rs, rs);
         T* yr = y + static_cast<int64_t>(row) * sh.cols;
 #pragma unroll
@@ -1160,13 +1158,8 @@ bool fwd_rows(WbBackend* b, const T* x, int64_t pitch, const Shape& s, const T* 
     return choose_row<MOST / VEC, 8>((s.cols + VEC - 1) / VEC, [&](auto tpr, auto nv) {
         constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, G = fwd_threads<TPR> / TPR;
         const int64_t grid = (s.rows + G - 1) / G;
-        if (grid > INT32_MAX) {
-            *err = cudaErrorInvalidConfiguration;
-            return;
-        }
         *err = wb_launch_pdl(ln_fwd_rows_kernel<T, VEC, TPR, NV>, dim3(static_cast<unsigned>(grid)), dim3(fwd_threads<TPR>), 0, b->stream, x, pitch,
-                             s.rows, static_cast<int>(s.cols), w, bias, static_cast<T>(eps), static_cast<T>(1.0 / static_cast<double>(s.cols)), y, mean,
-                             rstd);
+                             s.rows, static_cast<int>(s.cols), w, bias, static_cast<T>(eps), y, mean, rstd);
     });
 }
 
@@ -1384,8 +1377,7 @@ bool fwd_spans(WbBackend* b, const T* x, int64_t pitch, const Shape& s, const T*
         sh.ring = ring_depth(slots, CL);
         int slabs = 0;
         *err = launch_spans<ln_fwd_span_kernel<T, NV, CL, decltype(mode)::value>, CL>(b, sh, 1, slots * sh.ring, per, 0, &slabs, x, sh, w, bias,
-                                                                                     static_cast<T>(eps), static_cast<T>(1.0 / static_cast<double>(s.cols)),
-                                                                                     y, mean, rstd);
+                                                                                     static_cast<T>(eps), y, mean, rstd);
         return true;
     };
     auto wide = [&](auto mode) {
