@@ -152,12 +152,21 @@ __device__ __forceinline__ void row_sum(T (&v)[K], T* part, int bar, unsigned in
     }
 }
 
+// s / n, correctly rounded, from y = 1 / n correctly rounded: the quotient's exact residual corrects it (Markstein's theorem, as
+// in adam_multi.cu).  The mean of equal values then is that value where their sum is exact, which s y misses by a unit, and a
+// division in its place made the forward pass of [8192, 4096] in f64 107 us instead of 83.
+template <class T>
+__device__ __forceinline__ T divide(T s, T n, T y) {
+    const T q = s * y, r = fma(-q, n, s);
+    return r == r ? fma(r, y, q) : q;  // the residual of what is not finite is NaN
+}
+
 template <int TPR>
 constexpr int fwd_threads = TPR < 64 ? 128 : TPR;
 
 template <class T, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* __restrict__ x, int64_t pitch, int64_t rows, int cols,
-                                                                       const T* __restrict__ w, const T* __restrict__ bias, T eps,
+                                                                       const T* __restrict__ w, const T* __restrict__ bias, T eps, T inv_cols,
                                                                        T* __restrict__ y, T* __restrict__ mean_out, T* __restrict__ rstd_out) {
     constexpr int G = fwd_threads<TPR> / TPR;
     __shared__ T part[G][TPR > 32 ? 2 * TPR / 32 : 1];
@@ -181,7 +190,7 @@ __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* 
     }
     unsigned int turn = 0;
     row_sum<T, TPR, G, 1>(s, part[group], 1 + group, turn);
-    const T n = static_cast<T>(cols), mean = s[0] / n;  // a division: the mean of equal values is that value where their sum is exact
+    const T mean = divide(s[0], static_cast<T>(cols), inv_cols);
     T q[1] = {0};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -193,7 +202,7 @@ __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* 
         }
     }
     row_sum<T, TPR, G, 1>(q, part[group], 1 + group, turn);
-    const T rstd = T(1) / sqrt(q[0] / n + eps);
+    const T rstd = T(1) / sqrt(q[0] * inv_cols + eps);
     if (!live) return;
     T* yr = y + row * cols;
 #pragma unroll
@@ -827,8 +836,8 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
 // [4096, 12000] 98 us against 69 us, [4096, 16384] 115 against 98 us.
 template <class T, int NV, int CL, int MODE>
 __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_fwd_span_kernel(const T* __restrict__ x, const SpanShape sh, const T* __restrict__ w,
-                                                                     const T* __restrict__ bias, T eps, T* __restrict__ y, T* __restrict__ mean_out,
-                                                                     T* __restrict__ rstd_out) {
+                                                                     const T* __restrict__ bias, T eps, T inv_cols, T* __restrict__ y,
+                                                                     T* __restrict__ mean_out, T* __restrict__ rstd_out) {
     constexpr int TPR = SPAN_THREADS, U = UNIT<T>, H = U / 2;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ T part[2 * TPR / 32];
@@ -910,7 +919,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_fwd_span_kernel(const T* _
         settle(sh.ring - 2);
         row_sum<T, TPR, 1, 1>(s, part, 1, turn, [&]() { fetch(row + sh.ring * groups, slot); });
         if constexpr (CL > 1) cluster_sum<T, CL, 1>(s, peers, rank, turn);
-        const T n = static_cast<T>(sh.cols), mu = s[0] / n;
+        const T mu = divide(s[0], static_cast<T>(sh.cols), inv_cols);
         const Pair<T> minus_mu = pair(-mu, -mu);
         s2 = pair(T(0), T(0));
 #pragma unroll
@@ -925,7 +934,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_fwd_span_kernel(const T* _
         s[0] = lo + hi;
         row_sum<T, TPR, 1, 1>(s, part, 1, turn);
         if constexpr (CL > 1) cluster_sum<T, CL, 1>(s, peers, rank, turn);
-        const T rs = T(1) / sqrt(s[0] / n + eps);
+        const T rs = T(1) / sqrt(s[0] * inv_cols + eps);
         const Pair<T> rs2 = pair(rs, rs);
         T* yr = y + static_cast<int64_t>(row) * sh.cols;
 #pragma unroll
@@ -981,8 +990,9 @@ __global__ void __launch_bounds__(THREADS) ln_dw_any_kernel(const T* __restrict_
 }
 
 // Sums the slabs of both partial arrays: 32 columns per block, LINES lines of threads that take every LINES-th slab, joined in
-// order.  A line's loads are all in flight at once (ten: 32 lines reach 320 slabs, eight 80, four 40); 296 slabs by eight lines, their loads
-// in turn, took 10 us whatever the size, and 8 slabs of 16384 columns by 32 lines as long.
+// order.  A line's loads are all in flight at once (ten: 32 lines reach 320 slabs, eight 80, four 40); 296 slabs by eight lines,
+// their loads in turn, took 10 us whatever the size, 148 by eight lines of 20 loads 7.8 us against 4.9 us by 32 (the f64 additions
+// are a chain), and 8 slabs of 16384 columns by 32 lines 10 us.
 template <class T, int LINES>
 __global__ void __launch_bounds__(32 * LINES) ln_dw_join_kernel(const T* __restrict__ parts, int slabs, int64_t cols, T* __restrict__ dw,
                                                                 T* __restrict__ db) {
@@ -1159,7 +1169,8 @@ bool fwd_rows(WbBackend* b, const T* x, int64_t pitch, const Shape& s, const T* 
         constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, G = fwd_threads<TPR> / TPR;
         const int64_t grid = (s.rows + G - 1) / G;
         *err = wb_launch_pdl(ln_fwd_rows_kernel<T, VEC, TPR, NV>, dim3(static_cast<unsigned>(grid)), dim3(fwd_threads<TPR>), 0, b->stream, x, pitch,
-                             s.rows, static_cast<int>(s.cols), w, bias, static_cast<T>(eps), y, mean, rstd);
+                             s.rows, static_cast<int>(s.cols), w, bias, static_cast<T>(eps), static_cast<T>(1.0 / static_cast<double>(s.cols)), y, mean,
+                             rstd);
     });
 }
 
@@ -1377,7 +1388,8 @@ bool fwd_spans(WbBackend* b, const T* x, int64_t pitch, const Shape& s, const T*
         sh.ring = ring_depth(slots, CL);
         int slabs = 0;
         *err = launch_spans<ln_fwd_span_kernel<T, NV, CL, decltype(mode)::value>, CL>(b, sh, 1, slots * sh.ring, per, 0, &slabs, x, sh, w, bias,
-                                                                                     static_cast<T>(eps), y, mean, rstd);
+                                                                                     static_cast<T>(eps), static_cast<T>(1.0 / static_cast<double>(s.cols)),
+                                                                                     y, mean, rstd);
         return true;
     };
     auto wide = [&](auto mode) {
