@@ -9,8 +9,9 @@
 // carry the update, are kept to 0.8 % (m) and 0.4 % (sqrt(v)) and the least one is 6e-5 (1.5e-5) of the largest.
 // sqrt(v) rather than v is coded because it has m's range (v's is twice as many decades) and is at hand in the update.
 // A second moment that is not zero keeps at least code 1: rounding it to zero would leave m / (0 + eps).
-// Compiled with -fmad=false and without approximate functions: every f32 rounding is the one written here, so the
-// codes do not depend on the launch's shape, and the 32-bit step gives wb_adam_step's bits.
+// Compiled with -fmad=false, and approximate functions are corrected to the rounded result wherever it counts: every f32
+// rounding is the one written here, so the codes do not depend on the launch's shape, and the 32-bit step gives
+// wb_adam_step's bits.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -242,8 +243,9 @@ struct AdamK8 {
 };
 
 // One warp takes a block of 256 elements, a lane the groups of four at 4 lane and 128 + 4 lane.
-// Bound by instruction issue until the conversions left the conversion unit, the arithmetic went to pairs and a block took
-// a longer chunk (101 M elements in 128 tensors: 562 -> 293 us).
+// Bound by instruction issue (81 % of the slots): 101 M elements in 128 tensors took 562 us with conversions, roots and
+// quotients one at a time, 293 us now (251 us are their bytes).  One block per warp and five thread blocks per processor: with
+// two blocks in turn per warp 378 us, with four thread blocks 334 us, with six 322 us against 311 us at that stage.
 template <int N, bool FIRST>
 __global__ void __launch_bounds__(THREADS, 5) adam_multi8_kernel(const __grid_constant__ Table<N> tab, uint32_t* __restrict__ mc, uint32_t* __restrict__ vc,
                                                               float* __restrict__ ms, float* __restrict__ vs, const __grid_constant__ AdamK8 k8,
