@@ -385,6 +385,22 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ int cluster_size() {
+    uint32_t n;
+    asm("mov.u32 %0, %cluster_nctaid.x;" : "=r"(n));
+    return static_cast<int>(n);
+}
+// The value at the same place in the shared memory of the cluster's CTA q.
+template <class T>
+__device__ __forceinline__ T peer_value(const T* p, int q) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(q));
+    T v;
+    if constexpr (sizeof(T) == 4) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    else asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
+    return v;
+}
+
 // Adds the CTAs' sums of a row over the cluster: every CTA's to every CTA; two buffers in turn, as in row_sum.
 template <class T, int CL, int K>
 __device__ __forceinline__ void cluster_sum(T (&s)[K], T (*peers)[CL][2], int rank, unsigned int turn) {
@@ -609,7 +625,9 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
     if (!parts) return;
     __syncthreads();
     // one line for each row that the block holds at a time, added up in order
-    T* joined = reinterpret_cast<T*>(smem_raw);  // [2][LINES][TPR E]
+    T* joined = reinterpret_cast<T*>(smem_raw);  // [2][LINES][TPR E], then (a cluster's blocks) the block's sums [2][cols]
+    T* sums = joined + 2 * LINES * TPR * E;
+    const bool cluster = cluster_size() > 1;
     const int line = threadIdx.x / TPR;
     if (col.t == 0) line_mis[line] = col.mis;
 #pragma unroll
@@ -637,7 +655,10 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
             sw += a[0];
             sb += a[LINES * TPR * E];
         }
-        if (slabs == 1) {  // nothing to join
+        if (cluster) {
+            sums[c] = sw;
+            sums[sh.cols + c] = sb;
+        } else if (slabs == 1) {  // nothing to join
             if (dw) dw[c] = sw;
             if (db) db[c] = sb;
         } else {
@@ -645,6 +666,18 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
             parts[static_cast<int64_t>(slabs + slab) * sh.cols + c] = sb;
         }
     }
+    if (!cluster) return;
+    cluster_sync();  // every block's sums are there; each block adds up its share of the columns, in the blocks' order
+    for (int c = slab * N + static_cast<int>(threadIdx.x); c < sh.cols; c += slabs * N) {
+        T sw = 0, sb = 0;
+        for (int q = 0; q < slabs; ++q) {
+            sw += peer_value(sums + c, q);
+            sb += peer_value(sums + sh.cols + c, q);
+        }
+        if (dw) dw[c] = sw;
+        if (db) db[c] = sb;
+    }
+    cluster_sync();  // no block leaves while its sums are read
 }
 
 // Backward of rows wider than 512 threads hold: a cluster of CTAs takes the row, each its slice of the columns, and they
@@ -1209,10 +1242,12 @@ cudaError_t allow_shared(int ordinal) {
 }
 
 // The grid of a span kernel: as many groups as the device holds at a time or as there are spans, and a multiple of the
-// period, so that a group's rows are all of one misalignment; one slab where `few` spans per group let it do.  Then the launch,
-// as the programmatic dependent of what is before it.
+// period, so that a group's rows are all of one misalignment.  Where one block with at most `few` spans per group will do, or
+// up to `joint` of them, they leave the sums themselves, the latter as a cluster, and *slabs is 1: that saves the launch that
+// joins the partials, about what two more rows in turn take.  Then the launch, as the programmatic dependent of what is
+// before it.
 template <auto KERNEL, int CL, class... Args>
-cudaError_t launch_spans(WbBackend* b, const SpanShape& sh, int groups, size_t smem, int period, int few, int* slabs, Args... args) {
+cudaError_t launch_spans(WbBackend* b, const SpanShape& sh, int groups, size_t smem, int period, int few, int joint, int* slabs, Args... args) {
     cudaError_t e = allow_shared<KERNEL>(b->ordinal);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -1238,8 +1273,14 @@ cudaError_t launch_spans(WbBackend* b, const SpanShape& sh, int groups, size_t s
     int64_t want = std::min<int64_t>(most, (static_cast<int64_t>(sh.spans) + groups - 1) / groups);
     want = std::min((want + step - 1) / step * step, most / step * step);
     if (step == 1 && sh.spans <= few * groups) want = 1;
-    *slabs = static_cast<int>(std::max<int64_t>(want, step));
-    cfg.gridDim = dim3(static_cast<unsigned>(*slabs * CL));
+    else if (sh.spans <= few * joint * groups) want = std::min<int64_t>(want, joint / step * step);
+    want = std::max<int64_t>(want, step);
+    cfg.gridDim = dim3(static_cast<unsigned>(want * CL));
+    *slabs = static_cast<int>(want);
+    if (CL == 1 && want > 1 && want <= joint) {
+        attr[n++] = cluster_attribute(static_cast<unsigned>(want));
+        *slabs = 1;
+    }
     if (wb_pdl_allowed()) {
         attr[n] = cudaLaunchAttribute{};
         attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1315,11 +1356,10 @@ bool bwd_spans(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t p
         sh.r = GT == 32 && dense && (MODE == ALIGNED || MODE == ELEMENTS) ? rows_per_span<T>(b, s, G, SUBS) : 1;
         sh.spans = static_cast<int>((s.rows + sh.r - 1) / sh.r);
         sh.cap = buffer(sh.r * s.cols);
-        const size_t slots = sizeof(T) * static_cast<size_t>(G) * (2 * sh.cap + 64), join = sizeof(T) * 2 * N * NV * UNIT<T>;
+        const size_t slots = sizeof(T) * static_cast<size_t>(G) * (2 * sh.cap + 64), join = sizeof(T) * 2 * (N * NV * UNIT<T> + static_cast<size_t>(s.cols));
         sh.ring = ring_depth(slots, 1);
-        // one slab saves the launch that joins the partials, about what two more rows in a row take
         *err = launch_spans<ln_bwd_span_kernel<T, TPR, NV, MODE>, 1>(b, sh, G, std::max(slots * sh.ring, join), MODE == ELEMENTS ? 1 : per, parts ? 3 : 0,
-                                                                    slabs, x, dy, sh, w, mean, rstd, inv_cols, ref, dx, parts, dw, db);
+                                                                    parts ? 8 : 0, slabs, x, dy, sh, w, mean, rstd, inv_cols, ref, dx, parts, dw, db);
     };
     auto go_wide = [&](auto cl, auto mode) {
         constexpr int CL = decltype(cl)::value, MODE = decltype(mode)::value;
@@ -1329,7 +1369,7 @@ bool bwd_spans(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t p
         sh.cap = buffer(static_cast<int64_t>(sh.units) * UNIT<T>);
         const size_t slots = sizeof(T) * (2 * sh.cap + 64);
         sh.ring = 3;
-        *err = launch_spans<ln_bwd_wide_kernel<T, CL, MODE>, CL>(b, sh, 1, slots * sh.ring, per, parts ? 2 : 0, slabs, x, dy, sh, w, mean, rstd, inv_cols,
+        *err = launch_spans<ln_bwd_wide_kernel<T, CL, MODE>, CL>(b, sh, 1, slots * sh.ring, per, parts ? 2 : 0, 0, slabs, x, dy, sh, w, mean, rstd, inv_cols,
                                                                 ref, dx, parts, dw, db);
         return true;
     };
@@ -1387,7 +1427,7 @@ bool fwd_spans(WbBackend* b, const T* x, int64_t pitch, const Shape& s, const T*
         const size_t slots = sizeof(T) * static_cast<size_t>(sh.cap);
         sh.ring = ring_depth(slots, CL);
         int slabs = 0;
-        *err = launch_spans<ln_fwd_span_kernel<T, NV, CL, decltype(mode)::value>, CL>(b, sh, 1, slots * sh.ring, per, 0, &slabs, x, sh, w, bias,
+        *err = launch_spans<ln_fwd_span_kernel<T, NV, CL, decltype(mode)::value>, CL>(b, sh, 1, slots * sh.ring, per, 0, 0, &slabs, x, sh, w, bias,
                                                                                      static_cast<T>(eps), static_cast<T>(1.0 / static_cast<double>(s.cols)),
                                                                                      y, mean, rstd);
         return true;
