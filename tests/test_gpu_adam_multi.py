@@ -154,6 +154,24 @@ def test_steps_bit_for_bit(gpu, name, bits, wd, decoupled):
         assert same(m[o:o + p.n], want[0][:p.n]) and same(v[o:o + p.n], want[1][:p.n])
 
 
+@pytest.mark.parametrize("count", [32, 33, 128, 129, 320, 321, 768, 769])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_numbers_of_tensors_at_which_the_table_changes(gpu, count, bits):
+    lens = [(97 * k) % 301 for k in range(count)]
+    rng = np.random.default_rng(count)
+    thetas, gs = [rng.standard_normal(n).astype(F) for n in lens], grads_for(rng, lens)
+    stores = [gpu.from_host(t) if t.size else gpu.wrap_pointer(gpu.zeros(1, DType.F32).ptr, 0, DType.F32) for t in thetas]
+    opt = optim.AdamMulti(gpu, stores, bits, lr=3e-3, betas=(0.9, 0.99), eps=1e-8)
+    opt.set_grads([gpu.from_host(g) if g.size else None for g in gs])
+    plain = [Plain(n, bits) for n in lens]
+    for t in (1, 2):
+        opt.step(t)
+        thetas = [p.step(th, g, t, 3e-3, 0.9, 0.99, 1e-8, 0.0, False, False, None) for p, th, g in zip(plain, thetas, gs)]
+    assert all(same(down(gpu, s, n), th) for s, th, n in zip(stores, thetas, lens) if n)
+    want = math.sqrt(sum((g.astype(np.float64) ** 2).sum() for g in gs))
+    assert abs(float(down(gpu, opt.grad_norm(1.0)[0], 1)[0]) - want) <= 1.001 * U * want
+
+
 @pytest.mark.parametrize("shift", [0, 1, 2, 3])
 def test_32_bits_are_those_of_the_single_tensor_step(gpu, shift):
     """Tensors packed without padding, from an offset of `shift` elements, gradients at another alignment."""

@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(THREADS) grad_norm_kernel(const __grid_constan
 
 // ---- the handle ---------------------------------------------------------------------------------------------
 
-constexpr int SMALL = 32, LARGE = 768;  // tensors per launch: 1.5 KB and 28 KB of parameters (limit: 32,764 bytes)
+constexpr int LARGE = 768;  // tensors of a launch at most: 28 KB of arguments (limit: 32,764 bytes)
 static_assert(sizeof(Table<LARGE>) + sizeof(AdamK8) + 64 <= 32764, "a launch's parameters");
 
 int64_t padded(int64_t n) { return (n + BLOCK8 - 1) / BLOCK8 * BLOCK8; }
@@ -549,22 +549,34 @@ struct WbAdamMulti {
 
 namespace {
 
+// The smallest table that holds a launch's tensors, because all arguments are copied with every launch. A call on
+// tensors of 64 elements, f32 state, in a stream of calls: 33 tensors 6.5 us with the table of 768, 3.9 us with that
+// of 128; 300 tensors 6.4 and 4.8 us (320).
+template <int N, class F>
+int with_table(const Table<LARGE>& t, int l, F&& launch) {
+    if constexpr (N == LARGE) {
+        return launch(l, t);
+    } else {
+        Table<N> s;
+        s.n = t.n;
+        s.shift = t.shift;
+        s.chunks = t.chunks;
+        std::copy(t.hint, t.hint + HINTS + 1, s.hint);
+        std::copy(t.first, t.first + t.n, s.first);
+        std::copy(t.t, t.t + t.n, s.t);
+        return launch(l, s);
+    }
+}
+
 template <class F>
 int per_launch(WbAdamMulti* h, F&& launch) {
     for (size_t l = 0; l < h->launches.size(); ++l) {
         const Table<LARGE>& t = h->launches[l];
-        if (t.n <= SMALL) {
-            Table<SMALL> s;
-            s.n = t.n;
-            s.shift = t.shift;
-            s.chunks = t.chunks;
-            std::copy(t.hint, t.hint + HINTS + 1, s.hint);
-            std::copy(t.first, t.first + t.n, s.first);
-            std::copy(t.t, t.t + t.n, s.t);
-            WB_TRY(launch(static_cast<int>(l), s));
-        } else {
-            WB_TRY(launch(static_cast<int>(l), t));
-        }
+        const int i = static_cast<int>(l);
+        WB_TRY(t.n <= 32    ? with_table<32>(t, i, launch)
+               : t.n <= 128 ? with_table<128>(t, i, launch)
+               : t.n <= 320 ? with_table<320>(t, i, launch)
+                            : with_table<LARGE>(t, i, launch));
     }
     return WB_OK;
 }
