@@ -160,6 +160,37 @@ def test_values_that_are_not_finite_stay_in_their_row(gpu, cols):
     assert np.isnan(dx[bad]).all() and np.isfinite(dx[good]).all()
 
 
+def kind(a):
+    """0 finite, 1 and -1 the infinities, 2 NaN."""
+    return np.where(np.isnan(a), 2, np.where(np.isinf(a), np.sign(a), 0))
+
+
+@pytest.mark.parametrize("cols", [21, 36, 40, 131, 200, 520, 777, 1544, 3080, 5001, 9000, 9001, 17000])
+@pytest.mark.parametrize("dt", [DType.F32, DType.F64])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_an_infinite_gradient_reaches_what_the_formula_says(gpu, cols, dt, shift):
+    """An infinity in dy makes the row's dx infinite or NaN by the signs in the formula, and nothing else: a thread's places
+    behind the row's end add nothing, not zero times the infinity.  `shift`: dy starts an element behind x's alignment."""
+    rng = np.random.default_rng(cols + shift)
+    rows = 6
+    x, dy = (rng.standard_normal((rows, cols)).astype(NP[dt]) for _ in range(2))
+    dy[1, 0], dy[2, cols - 1], dy[4, cols // 2] = np.inf, -np.inf, np.inf
+    w = rng.uniform(0.5, 1.5, cols).astype(NP[dt])
+    l = Layout.contiguous([rows, cols])
+    sx, sw = gpu.from_host(x.reshape(-1)), gpu.from_host(w)
+    sg = gpu.from_host(np.concatenate([np.zeros(shift, NP[dt]), dy.reshape(-1)]))
+    _, mean, rstd = layers.layer_norm_fwd(gpu, sx, l, dt, 1, sw)
+    dx, dw, db = layers.layer_norm_bwd(gpu, sx, l, sg, Layout([rows, cols], [cols, 1], shift), dt, 1, sw, mean, rstd)
+    got = [get(gpu, a, b, dt) for a, b in ((dx, (rows, cols)), (dw, (cols,)), (db, (cols,)))]
+    m, r = (get(gpu, a, (rows, 1), dt).astype(np.longdouble) for a in (mean, rstd))
+    with np.errstate(invalid="ignore"):
+        xh = (x.astype(np.longdouble) - m) * r
+        g = dy.astype(np.longdouble) * w
+        want = (r * (g - g.sum(1, keepdims=True) - xh * (g * xh).sum(1, keepdims=True)), (dy * xh).sum(0), dy.astype(np.longdouble).sum(0))
+    for a, b in zip(got, want):
+        assert np.array_equal(kind(a), kind(b))
+
+
 VIEWS = {  # name: (storage length, Layout, normalised dims)
     "two normalised dims": (5 * 6 * 7, Layout.contiguous([5, 6, 7]), 2),
     "all dims": (6 * 7, Layout.contiguous([6, 7]), 2),

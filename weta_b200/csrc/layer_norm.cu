@@ -444,6 +444,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
     __shared__ T part[G][TPR > 32 ? 4 * TPR / 32 : 1];
     __shared__ uint64_t full[G][MOST_RING];
     __shared__ int line_mis[LINES];
+    __shared__ alignas(16) T zeros[U];
     wb_pdl_enter();
     const int group = threadIdx.x / GT, g = threadIdx.x % GT, sub = g / TPR;
     const int slab = static_cast<int>(blockIdx.x), slabs = static_cast<int>(gridDim.x);
@@ -459,6 +460,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
     const int slot_elems = 2 * sh.cap + 64;
     T* ring = reinterpret_cast<T*>(smem_raw) + group * sh.ring * slot_elems + U;
     if (g < sh.ring) bar_init(&full[group][g]);
+    if (threadIdx.x < U) zeros[threadIdx.x] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncthreads();
     if constexpr (MODE == SHIFTED) {  // the ends of each buffer: a unit before and after the first, all from the last on
@@ -552,16 +554,18 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
                     Pair<T> up[H];
                     if constexpr (MODE == ELEMENTS) {
 #pragma unroll
-                        for (int i = 0; i < H; ++i) {  // behind the row's end: its last element, which has no weight there
-                            const int c = min(column(j, 2 * i), sh.cols - 1), d = min(column(j, 2 * i + 1), sh.cols - 1);
-                            xh[j][i] = pair(bx[c], bx[d]);
-                            up[i] = pair(bg[c], bg[d]);
+                        for (int i = 0; i < H; ++i) {
+                            const int c = column(j, 2 * i), d = column(j, 2 * i + 1);
+                            const bool a = c < sh.cols, b = d < sh.cols;
+                            xh[j][i] = pair(a ? bx[c] : T(0), b ? bx[d] : T(0));
+                            up[i] = pair(a ? bg[c] : T(0), b ? bg[d] : T(0));
                         }
                     } else {
-                        // a unit behind the row's end (of the last vector only, in a row of its own): any that is there
-                        const int at = j < NV - 1 || col.some(j) ? j * TPR * U : -col.t * U;
-                        load_unit<T, MODE != MIXED>(bx + at, xh[j]);
-                        load_unit<T, MODE != MIXED>(bg + at, up);
+                        // a unit behind the row's end (of the last vector only, in a row of its own): zeros, since no weight makes
+                        // nothing of an infinity
+                        const bool there = j < NV - 1 || col.some(j);
+                        load_unit<T, MODE != MIXED>(there ? bx + j * TPR * U : zeros, xh[j]);
+                        load_unit<T, MODE != MIXED>(there ? bg + j * TPR * U : zeros, up);
                     }
                     if constexpr (decltype(edges)::value) {  // what is not of this row counts as a mean value without gradient
                         replace_outside(col.first(j), sh.cols, mu, xh[j]);
@@ -693,6 +697,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
     __shared__ T part[4 * TPR / 32];
     __shared__ T peers[2][CL][2];
     __shared__ uint64_t full[MOST_RING];
+    __shared__ alignas(16) T zeros[U];
     wb_pdl_enter();
     const int t = threadIdx.x, rank = static_cast<int>(blockIdx.x) % CL, slab = static_cast<int>(blockIdx.x) / CL, slabs = static_cast<int>(gridDim.x) / CL;
     Columns<T, TPR, NV> col;
@@ -705,6 +710,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
     const int slot_elems = 2 * sh.cap + 64;  // see ln_bwd_span_kernel
     T* ring = reinterpret_cast<T*>(smem_raw) + U;
     if (t < sh.ring) bar_init(&full[t]);
+    if (t < U) zeros[t] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncthreads();
     cluster_sync();
@@ -747,14 +753,14 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
     };
     // xhat and dy of unit j of a row in a slot
     auto load = [&](int row, int slot, int j, T mu, const Pair<T>& minus_mu, const Pair<T>& rs2, Pair<T>(&xh)[H], Pair<T>(&up)[H]) {
-        const T* base = ring + slot * slot_elems + col.u0 * U - col.mis - from + t * U + (col.some(j) ? j * TPR * U : -t * U);
+        const T* base = ring + slot * slot_elems + col.u0 * U - col.mis - from + (j * TPR + t) * U;
         int mx = 0, mg = 0;
         if (MODE != ALIGNED) {
             mx = misalignment(x + row * sh.pitch_x + from);
             mg = misalignment(dy + row * sh.pitch_g + from);
         }
-        load_unit<T, MODE != MIXED>(base + mx, xh);
-        load_unit<T, MODE != MIXED>(base + sh.cap + mg, up);
+        load_unit<T, MODE != MIXED>(col.some(j) ? base + mx : zeros, xh);
+        load_unit<T, MODE != MIXED>(col.some(j) ? base + sh.cap + mg : zeros, up);
         if (MODE == MIXED && !whole) {
             replace_outside(col.first(j), to, mu, xh);
             replace_outside(col.first(j), to, T(0), up);
