@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
                             if (column(j, 2 * i + 1) < sh.cols) dr[column(j, 2 * i + 1)] = b;
                         }
                     } else if (MODE == ALIGNED ? j < NV - 1 || col.some(j) : whole || col.whole(j)) store_unit(dr + col.first(j), o);
-                    else if (MODE != ALIGNED) store_part(dr, col.first(j), sh.cols, o);
+                    else if (MODE != ALIGNED && (j < NV - 1 || col.some(j))) store_part(dr, col.first(j), sh.cols, o);
                 }
             }
         }
@@ -687,12 +687,12 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
 // Backward of rows wider than 512 threads hold: a cluster of CTAs takes the row, each its slice of the columns, and they
 // exchange the two sums.  A row goes through two passes over its slot, the first for the sums and the columns' gradients, the
 // second for dx; the cluster's barrier for one row is waited for only after the next row's first pass, which hides it.
-template <class T, int CL, int MODE>
+template <class T, int NV, int CL, int MODE>
 __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* __restrict__ x, const T* __restrict__ dy, const SpanShape sh,
                                                                      const T* __restrict__ w, const T* __restrict__ mean,
                                                                      const T* __restrict__ rstd, T inv_cols, const T* ref, T* __restrict__ dx,
                                                                      T* __restrict__ parts, T* __restrict__ dw, T* __restrict__ db) {
-    constexpr int TPR = SPAN_THREADS, NV = 4, U = UNIT<T>, H = U / 2;
+    constexpr int TPR = SPAN_THREADS, U = UNIT<T>, H = U / 2;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ T part[4 * TPR / 32];
     __shared__ T peers[2][CL][2];
@@ -840,7 +840,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
 #pragma unroll
                     for (int i = 0; i < H; ++i) o[i] = muladd(up[i] * wv[j][i], rs2, muladd(xh[i], k1p, k0p));
                     if (whole || col.whole(j)) store_unit(dr + col.first(j), o);
-                    else if (MODE != ALIGNED) store_part(dr, col.first(j), to, o);
+                    else if (MODE != ALIGNED && col.some(j)) store_part(dr, col.first(j), to, o);
                 }
             }
         }
@@ -982,7 +982,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_fwd_span_kernel(const T* _
 #pragma unroll
             for (int i = 0; i < H; ++i) o[i] = muladd(d[j][i] * rs2, wv[j][i], bv[j][i]);
             if (whole || col.whole(j)) store_unit(yr + col.first(j), o);
-            else if (MODE != ALIGNED) store_part(yr, col.first(j), to, o);
+            else if (MODE != ALIGNED && col.some(j)) store_part(yr, col.first(j), to, o);
         }
         if (t == 0 && rank == 0) {
             if (mean_out) mean_out[row] = mu;
@@ -1367,15 +1367,15 @@ bool bwd_spans(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t p
         *err = launch_spans<ln_bwd_span_kernel<T, TPR, NV, MODE>, 1>(b, sh, G, std::max(slots * sh.ring, join), MODE == ELEMENTS ? 1 : per, parts ? 3 : 0,
                                                                     parts ? 8 : 0, slabs, x, dy, sh, w, mean, rstd, inv_cols, ref, dx, parts, dw, db);
     };
-    auto go_wide = [&](auto cl, auto mode) {
-        constexpr int CL = decltype(cl)::value, MODE = decltype(mode)::value;
+    auto go_wide = [&](auto nv, auto cl, auto mode) {
+        constexpr int NV = decltype(nv)::value, CL = decltype(cl)::value, MODE = decltype(mode)::value;
         sh.units = static_cast<int>((units + CL - 1) / CL);
         sh.r = 1;
         sh.spans = static_cast<int>(s.rows);
         sh.cap = buffer(static_cast<int64_t>(sh.units) * UNIT<T>);
         const size_t slots = sizeof(T) * (2 * sh.cap + 64);
         sh.ring = 3;
-        *err = launch_spans<ln_bwd_wide_kernel<T, CL, MODE>, CL>(b, sh, 1, slots * sh.ring, per, parts ? 2 : 0, 0, slabs, x, dy, sh, w, mean, rstd, inv_cols,
+        *err = launch_spans<ln_bwd_wide_kernel<T, NV, CL, MODE>, CL>(b, sh, 1, slots * sh.ring, per, parts ? 2 : 0, 0, slabs, x, dy, sh, w, mean, rstd, inv_cols,
                                                                 ref, dx, parts, dw, db);
         return true;
     };
@@ -1403,10 +1403,15 @@ bool bwd_spans(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t p
     });
     if (done) return true;
     auto wide = [&](auto mode) {
-        if (units <= 2 * 2048) return go_wide(std::integral_constant<int, 2>{}, mode);
-        if (units <= 4 * 2048) return go_wide(std::integral_constant<int, 4>{}, mode);
-        if (units <= 8 * 2048) return go_wide(std::integral_constant<int, 8>{}, mode);
-        return false;
+        // the fewest units per thread that hold the row: [4000, 9001] 129 us with three, 152 us with four; [4096, 12000] 125
+        // and 131 us
+        auto over = [&](auto cl) {
+            constexpr int CL = decltype(cl)::value;
+            if (units <= CL * 3 * SPAN_THREADS) return go_wide(std::integral_constant<int, 3>{}, cl, mode);
+            if (units <= CL * 4 * SPAN_THREADS) return go_wide(std::integral_constant<int, 4>{}, cl, mode);
+            return false;
+        };
+        return over(std::integral_constant<int, 2>{}) || over(std::integral_constant<int, 4>{}) || over(std::integral_constant<int, 8>{});
     };
     if (!same) return wide(std::integral_constant<int, MIXED>{});
     return cut ? wide(std::integral_constant<int, SHIFTED>{}) : wide(std::integral_constant<int, ALIGNED>{});
