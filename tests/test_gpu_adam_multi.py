@@ -541,3 +541,23 @@ def test_captured_clipped_steps(gpu, bits):
     del graph
     for arm in arms:
         arm[1].close()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_scalars_may_not_lie_in_what_the_step_writes(gpu, bits):
+    a, g = gpu.zeros(600, DType.F32), gpu.zeros(600, DType.F32)
+    opt = optim.AdamMulti(gpu, [a], bits)
+    opt.set_grads([g])
+    state_end = opt.state.ptr + opt.state_bytes - 4
+    for p in (a.ptr, a.ptr + 4 * 599, opt.state.ptr, state_end):
+        inside, fine = gpu.wrap_pointer(p, 1, DType.F32), gpu.zeros(1, DType.F32)
+        with pytest.raises(BackendError, match="lies in a parameter"):
+            opt.step(1, inside)
+        for out in ((inside, fine), (fine, inside)):
+            with pytest.raises(BackendError, match="lies in a parameter"):
+                opt.grad_norm(1.0, out=out)
+    with pytest.raises(BackendError, match="bytes each"):
+        opt.read_state(out=(gpu.zeros(100, DType.F32), None))
+    with pytest.raises(BackendError, match="not f32"):
+        optim.AdamMulti(gpu, [gpu.zeros(10, DType.F64)])
+    opt.step(1, fine)

@@ -226,7 +226,7 @@ def test_views(gpu, name, dt):
     rng = np.random.default_rng(len(name))
     store = (rng.standard_normal(length) + 0.2).astype(NP[dt])
     x = store[l.offsets()]
-    rows, cols = layers._rows_cols(l, nd)
+    rows, cols = l.rows_cols(nd)
     x = x.reshape(rows, cols)
     dense = Layout.contiguous(l.shape)
     other = rng.standard_normal((rows, cols)).astype(NP[dt])

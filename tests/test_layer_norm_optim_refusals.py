@@ -6,7 +6,7 @@ import ctypes
 import pytest
 
 from weta_b200 import layers, optim
-from weta_b200.backend import load_library
+from weta_b200.backend import BackendError, DeviceStorage, load_library
 from weta_b200.core import DType, Layout
 
 INVALID, UNSUPPORTED = 1, 2
@@ -150,3 +150,63 @@ def test_null_handles(lib, handle):
     assert lib.wb_adam_multi_grad_norm(None, 1.0, addr(1), None) == INVALID
     assert lib.wb_adam_multi_step(None, None, 1, 1.0, None) == INVALID
     assert lib.wb_adam_multi_read_state(None, addr(1), None) == INVALID
+
+
+class FakeLib:
+    """Fails the test where a call gets as far as the library."""
+    _wb_layers_declared = _wb_optim_declared = True
+
+    def __getattr__(self, name):
+        raise AssertionError(f"{name} was called")
+
+
+class FakeBackend:
+    lib, handle = FakeLib(), None
+
+
+def storage(n, dt=DType.F32):
+    s = DeviceStorage.__new__(DeviceStorage)
+    s.handle, s.backend, s.ptr, s._length, s._bytes = None, FakeBackend(), BASE, n, 0
+    s.backend.lib = FakeLib()
+    s.backend.lib.wb_storage_dtype = lambda handle: dt
+    return s
+
+
+@pytest.mark.parametrize("short", ["weight", "bias", "y", "mean", "rstd"])
+@pytest.mark.parametrize("dt", [DType.F32, DType.F64])
+def test_forward_refuses_short_storages(short, dt):
+    need = dict(weight=8, bias=8, y=32, mean=4, rstd=4)
+    s = {k: storage(n - (k == short), dt) for k, n in need.items()}
+    with pytest.raises(BackendError, match=f"{short} holds"):
+        layers.layer_norm_fwd(FakeBackend(), storage(32, dt), Layout.contiguous([4, 8]), dt, 1, s["weight"], s["bias"], out=(s["y"], s["mean"], s["rstd"]))
+
+
+@pytest.mark.parametrize("short", ["weight", "mean", "rstd", "dx", "dweight", "dbias"])
+@pytest.mark.parametrize("dt", [DType.F32, DType.F64])
+def test_backward_refuses_short_storages(short, dt):
+    need = dict(weight=8, mean=4, rstd=4, dx=32, dweight=8, dbias=8)
+    s = {k: storage(n - (k == short), dt) for k, n in need.items()}
+    l, x = Layout.contiguous([4, 8]), storage(32, dt)
+    with pytest.raises(BackendError, match=f"{short} holds"):
+        layers.layer_norm_bwd(FakeBackend(), x, l, x, l, dt, 1, s["weight"], s["mean"], s["rstd"], out=(s["dx"], s["dweight"], s["dbias"]),
+                              workspace=storage(1 << 20, dt))
+
+
+def test_a_storage_of_narrower_elements_is_too_short():
+    s, l = storage(64, DType.F64), Layout.contiguous([4, 8])
+    with pytest.raises(BackendError, match="weight holds 32 bytes, 64 are needed"):
+        layers.layer_norm_fwd(FakeBackend(), s, l, DType.F64, 1, storage(8), None, out=(s, s, s))
+
+
+def test_adam_refuses_storages_that_are_not_f32():
+    o = optim.AdamMulti.__new__(optim.AdamMulti)
+    o.be, o.lib, o.handle, o.params = FakeBackend(), FakeLib(), None, [storage(10)]
+    with pytest.raises(BackendError, match="gradient 0 is not f32"):
+        o.set_grads([storage(10, DType.F64)])
+    with pytest.raises(BackendError, match="gradient 0 has 9"):
+        o.set_grads([storage(9)])
+    for s in (storage(1, DType.F64), storage(0)):
+        with pytest.raises(BackendError, match="scale"):
+            o.step(1, s)
+    with pytest.raises(BackendError, match="norm"):
+        o.grad_norm(1.0, out=(storage(1), storage(0)))

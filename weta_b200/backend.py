@@ -102,19 +102,26 @@ def load_library():
 class DeviceStorage:
     """An owned WbStorage handle; returns its block to the backend's arena when collected."""
 
-    __slots__ = ("handle", "backend", "ptr", "_length", "__weakref__")
+    __slots__ = ("handle", "backend", "ptr", "_length", "_bytes", "__weakref__")
 
     def __init__(self, handle: int, backend: "B200Backend"):
         self.handle = handle
         self.backend = backend
         self.ptr = backend.lib.wb_storage_data(handle)  # neither address nor length changes while the handle lives
         self._length = None
+        self._bytes = 0  # not asked for yet
 
     @property
     def length(self) -> int:
         if self._length is None:
             self._length = self.backend.lib.wb_storage_len(self.handle)
         return self._length
+
+    @property
+    def nbytes(self) -> int:
+        if self._bytes == 0:
+            self._bytes = self.length * DType.size(self.backend.lib.wb_storage_dtype(self.handle))
+        return self._bytes
 
     def __del__(self):
         be = self.backend

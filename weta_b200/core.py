@@ -129,14 +129,14 @@ def contiguous_strides(shape: Sequence[int]) -> List[int]:
 class Layout:
     """crates/weta-core/src/layout.rs:16-21: shape, strides and offset, all in elements."""
 
-    __slots__ = ("shape", "strides", "offset", "_view")
+    __slots__ = ("shape", "strides", "offset", "_view", "_rows")
 
     def __init__(self, shape: Sequence[int], strides: Sequence[int], offset: int = 0):
         assert len(shape) == len(strides)
         self.shape = tuple(int(s) for s in shape)
         self.strides = tuple(int(s) for s in strides)
         self.offset = int(offset)
-        self._view = None
+        self._view = self._rows = None
 
     @staticmethod
     def contiguous(shape: Sequence[int]) -> "Layout":
@@ -148,6 +148,14 @@ class Layout:
 
     def numel(self) -> int:
         return math.prod(self.shape)
+
+    def rows_cols(self, inner_dims: int) -> Tuple[int, int]:
+        """The elements of the dims before the last `inner_dims`, and of those."""
+        r = self._rows
+        if r is None or r[0] != inner_dims:
+            outer = self.ndim - inner_dims
+            r = self._rows = (inner_dims, (math.prod(self.shape[:outer]), math.prod(self.shape[outer:])))
+        return r[1]
 
     def is_contiguous(self) -> bool:  # layout.rs:60-69
         expected = 1

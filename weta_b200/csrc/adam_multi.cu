@@ -549,6 +549,13 @@ struct WbAdamMulti {
 
 namespace {
 
+// Whether [lo, hi) touches a parameter or the state.
+bool touches(const WbAdamMulti* h, const void* p, int64_t bytes) {
+    const char *lo = static_cast<const char*>(p), *hi = lo + bytes;
+    auto it = std::lower_bound(h->thetas.begin(), h->thetas.end(), hi, [](const Range& r, const char* q) { return r.lo < q; });
+    return it != h->thetas.begin() && (it - 1)->hi > lo;
+}
+
 // The smallest table that holds a launch's tensors, because all arguments are copied with every launch. A call on
 // tensors of 64 elements, f32 state, in a stream of calls: 33 tensors 6.5 us with the table of 768, 3.9 us with that
 // of 128; 300 tensors 6.4 and 4.8 us (320).
@@ -692,9 +699,7 @@ extern "C" int wb_adam_multi_set_grads(WbAdamMulti* h, const float* const* grads
     for (int i = 0; i < n; ++i) {
         if (!grads[i] || h->lens[i] == 0) continue;
         WB_REQUIRE(reinterpret_cast<uintptr_t>(grads[i]) % 4 == 0, WB_ERR_INVALID, "wb_adam_multi_set_grads: gradient %d is not aligned to 4 bytes", i);
-        const char *lo = reinterpret_cast<const char*>(grads[i]), *hi = lo + 4 * h->lens[i];
-        auto it = std::lower_bound(h->thetas.begin(), h->thetas.end(), hi, [](const Range& r, const char* p) { return r.lo < p; });
-        WB_REQUIRE(it == h->thetas.begin() || (it - 1)->hi <= lo, WB_ERR_INVALID, "wb_adam_multi_set_grads: gradient %d overlaps a parameter or the state", i);
+        WB_REQUIRE(!touches(h, grads[i], 4 * h->lens[i]), WB_ERR_INVALID, "wb_adam_multi_set_grads: gradient %d overlaps a parameter or the state", i);
     }
     int i = 0;
     for (auto& t : h->launches)
@@ -708,6 +713,8 @@ extern "C" int wb_adam_multi_grad_norm(WbAdamMulti* h, double max_norm, float* n
     WB_REQUIRE(h->grads_set, WB_ERR_INVALID, "wb_adam_multi_grad_norm: no gradients were set");
     WB_REQUIRE((reinterpret_cast<uintptr_t>(norm) | reinterpret_cast<uintptr_t>(clip_scale)) % 4 == 0 && norm != clip_scale, WB_ERR_INVALID,
                "wb_adam_multi_grad_norm: the two outputs are one, or not aligned to 4 bytes");
+    WB_REQUIRE(!touches(h, norm, 4) && !(clip_scale && touches(h, clip_scale, 4)), WB_ERR_INVALID,
+               "wb_adam_multi_grad_norm: an output lies in a parameter or the state");
     WB_REQUIRE(!clip_scale || max_norm > 0.0, WB_ERR_INVALID, "wb_adam_multi_grad_norm: the largest norm has to be above 0, got %g", max_norm);
     WbBackend* b = h->b;
     WbDeviceGuard dev(b->ordinal);
@@ -732,6 +739,7 @@ extern "C" int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64
     WB_REQUIRE(h && cfg, WB_ERR_INVALID, "wb_adam_multi_step: null pointer");
     WB_REQUIRE(h->grads_set, WB_ERR_INVALID, "wb_adam_multi_step: no gradients were set");
     WB_REQUIRE(reinterpret_cast<uintptr_t>(device_grad_scale) % 4 == 0, WB_ERR_INVALID, "wb_adam_multi_step: the scale is not aligned to 4 bytes");
+    WB_REQUIRE(!device_grad_scale || !touches(h, device_grad_scale, 4), WB_ERR_INVALID, "wb_adam_multi_step: the scale lies in a parameter or the state");
     WB_REQUIRE(t >= 1 && t <= INT32_MAX, WB_ERR_INVALID, "wb_adam_multi_step: step counts from 1 to 2^31 - 1");
     WbBackend* b = h->b;
     WbDeviceGuard dev(b->ordinal);

@@ -1161,8 +1161,26 @@ struct SpanList {
 // launch_spans).
 int dw_slabs(int sm_count, int64_t rows) { return static_cast<int>(std::max<int64_t>(4, std::min<int64_t>((rows + 3) / 4 * 4, 2 * sm_count))); }
 
-// Unit stride along the row and one stride from row to row.
-bool plain_rows(const RowView& v, const Shape& s) { return v.nd_row == 1 && v.nd_col == 1 && (v.st_col[0] == 1 || s.cols == 1); }
+// Unit stride along the row and one stride, *pitch, from row to row (0 where there is one row).
+bool plain_rows(const WbView& v, int normalized_dims, int64_t* pitch) {
+    int64_t run = 1;
+    int d = v.ndim - 1;
+    for (; d >= v.ndim - normalized_dims; --d) {
+        if (v.shape[d] == 1) continue;
+        if (v.stride[d] != run) return false;
+        run *= v.shape[d];
+    }
+    *pitch = 0;
+    bool one = true;
+    for (; d >= 0; --d) {
+        if (v.shape[d] == 1) continue;
+        if (one) *pitch = run = v.stride[d];
+        else if (v.stride[d] != run) return false;
+        one = false;
+        run *= v.shape[d];
+    }
+    return true;
+}
 
 // 16-byte accesses: every row of every operand starts on a 16-byte boundary.
 template <class T>
@@ -1468,11 +1486,10 @@ bool fwd_spans(WbBackend* b, const T* x, int64_t pitch, const Shape& s, const T*
 template <class T>
 int fwd_typed(WbBackend* b, const WbView* x, int nd, const Shape& s, const T* w, const T* bias, double eps, T* y, T* mean, T* rstd) {
     const T* xp = reinterpret_cast<const T*>(view_data(*x));
-    const RowView vx = row_view(*x, nd);
     cudaError_t err = cudaSuccess;
     bool done = false;
-    if (plain_rows(vx, s) && s.rows < (1 << 30)) {
-        const int64_t pitch = vx.st_row[0];
+    int64_t pitch;
+    if (plain_rows(*x, nd, &pitch) && s.rows < (1 << 30)) {
         if (s.cols * static_cast<int64_t>(sizeof(T)) > 32768) done = fwd_spans<T>(b, xp, pitch, s, w, bias, eps, y, mean, rstd, &err);
         if (done) {
         } else if (rows_aligned<T>(xp, pitch, s.cols) && rows_aligned<T>(y, s.cols, s.cols) &&
@@ -1487,7 +1504,7 @@ int fwd_typed(WbBackend* b, const WbView* x, int nd, const Shape& s, const T* w,
     }
     if (!done) {
         const unsigned grid = static_cast<unsigned>(std::min<int64_t>(s.rows, 65535));
-        err = wb_launch_pdl(ln_fwd_any_kernel<T>, dim3(grid), dim3(THREADS), 0, b->stream, xp, vx, s.rows, s.cols, w, bias, eps, y, mean, rstd);
+        err = wb_launch_pdl(ln_fwd_any_kernel<T>, dim3(grid), dim3(THREADS), 0, b->stream, xp, row_view(*x, nd), s.rows, s.cols, w, bias, eps, y, mean, rstd);
     }
     WB_CHECK_CUDA(err);
     WB_LAUNCH_OK(b);
@@ -1499,18 +1516,23 @@ int bwd_typed(WbBackend* b, const WbView* x, const WbView* dy, int nd, const Sha
               T* parts) {
     const T* xp = reinterpret_cast<const T*>(view_data(*x));
     const T* gp = reinterpret_cast<const T*>(view_data(*dy));
-    const RowView vx = row_view(*x, nd), vg = row_view(*dy, nd);
     const bool sums = dw || db;
     if (!dx && !sums) return WB_OK;
     cudaError_t err = cudaSuccess;
     bool done = false;
     int slabs = dw_slabs(b->sm_count, s.rows);
-    if (plain_rows(vx, s) && plain_rows(vg, s) && s.rows < (1 << 30)) {
-        done = bwd_spans<T>(b, xp, vx.st_row[0], gp, vg.st_row[0], s, w, mean, rstd, dx, sums ? parts : nullptr, dw, db, &slabs, &err);
+    int64_t pitch_x, pitch_g;
+    if (plain_rows(*x, nd, &pitch_x) && plain_rows(*dy, nd, &pitch_g) && s.rows < (1 << 30)) {
+        done = bwd_spans<T>(b, xp, pitch_x, gp, pitch_g, s, w, mean, rstd, dx, sums ? parts : nullptr, dw, db, &slabs, &err);
         if (done) {
             WB_CHECK_CUDA(err);
             WB_LAUNCH_OK(b);
         }
+    }
+    RowView vx, vg;
+    if (!done) {
+        vx = row_view(*x, nd);
+        vg = row_view(*dy, nd);
     }
     if (!done && dx) {
         const unsigned grid = static_cast<unsigned>(std::min<int64_t>(s.rows, 65535));

@@ -1,7 +1,8 @@
 """Fused layer ops on device storages: layer normalisation, forward and backward (include/weta_b200.h `wb_layer_norm_*`).
 
 Tensors come as (storage, Layout, dtype), the way the backend's own methods take them; results are fresh contiguous
-storages from the backend's arena unless `out` gives them.
+storages from the backend's arena unless `out` gives them.  Storages that are taken whole are checked for their length; a
+view is not checked against its storage, as in the backend's methods.
 """
 from __future__ import annotations
 
@@ -29,18 +30,11 @@ def _declare(lib):
     lib._wb_layers_declared = True
 
 
-def _ptr(s: Optional[DeviceStorage]):
-    return None if s is None else s.ptr
-
-
-def _rows_cols(l: Layout, normalized_dims: int) -> Tuple[int, int]:
-    rows = cols = 1
-    for d, n in enumerate(l.shape):
-        if d < l.ndim - normalized_dims:
-            rows *= n
-        else:
-            cols *= n
-    return rows, cols
+def _too_short(what: str, dt: int, *needs: Tuple[str, Optional[DeviceStorage], int]):
+    """Refuses storages that hold fewer than so many elements of dtype `dt`."""
+    for name, s, n in needs:
+        if s is not None and s.nbytes < n * DType.size(dt):
+            raise BackendError(_INVALID, f"{what}: {name} holds {s.nbytes} bytes, {n * DType.size(dt)} are needed")
 
 
 def layer_norm_fwd(be: B200Backend, x: DeviceStorage, l: Layout, dt: int, normalized_dims: int, weight: Optional[DeviceStorage] = None,
@@ -50,16 +44,28 @@ def layer_norm_fwd(be: B200Backend, x: DeviceStorage, l: Layout, dt: int, normal
 
     `out` = (y, mean, rstd) writes there instead; mean and rstd may then be None, where no backward pass follows.
     """
-    _declare(be.lib)
-    v = l.view(x.ptr, dt)
-    if out is None:
-        if not 1 <= normalized_dims <= l.ndim or not DType.is_float(dt):
-            out = (x, None, None)  # refused below, with the library's message
-        else:
-            rows, _ = _rows_cols(l, normalized_dims)
-            out = (be.alloc(l.numel(), dt), be.alloc(rows, dt), be.alloc(rows, dt))
-    y, mean, rstd = out
-    be.check(be.lib.wb_layer_norm_fwd(be.handle, v, normalized_dims, _ptr(weight), _ptr(bias), eps, _ptr(y), _ptr(mean), _ptr(rstd)))
+    lib = be.lib
+    if not hasattr(lib, "_wb_layers_declared"):
+        _declare(lib)
+    if 1 <= normalized_dims <= len(l.shape) and (dt == DType.F32 or dt == DType.F64):
+        rows, cols = l.rows_cols(normalized_dims)
+        if out is None:
+            out = (be.alloc(rows * cols, dt), be.alloc(rows, dt), be.alloc(rows, dt))
+        y, mean, rstd = out
+        size = 4 if dt == DType.F32 else 8
+        # the lengths in bytes as far as they are known: those that are not read as 0, and _too_short asks for them
+        if ((weight is not None and weight._bytes < cols * size) or (bias is not None and bias._bytes < cols * size)
+                or (y is not None and y._bytes < rows * cols * size) or (mean is not None and mean._bytes < rows * size)
+                or (rstd is not None and rstd._bytes < rows * size)):
+            _too_short("layer norm", dt, ("weight", weight, cols), ("bias", bias, cols), ("y", y, rows * cols), ("mean", mean, rows),
+                       ("rstd", rstd, rows))
+    else:  # refused below, with the library's message
+        y, mean, rstd = x, None, None
+    status = lib.wb_layer_norm_fwd(be.handle, l.view(x.ptr, dt), normalized_dims, None if weight is None else weight.ptr,
+                                   None if bias is None else bias.ptr, eps, None if y is None else y.ptr, None if mean is None else mean.ptr,
+                                   None if rstd is None else rstd.ptr)
+    if status:
+        be.check(status)
     return y, mean, rstd
 
 
@@ -82,16 +88,29 @@ def layer_norm_bwd(be: B200Backend, x: DeviceStorage, lx: Layout, dy: DeviceStor
     given back after the call, which the arena orders on the backend's stream; a call that is captured into a CUDA
     graph brings its own and keeps it as long as the graph.
     """
-    _declare(be.lib)
-    vx, vg = lx.view(x.ptr, dt), ldy.view(dy.ptr, dt)
-    if (out is None or workspace is None) and 1 <= normalized_dims <= lx.ndim and DType.is_float(dt):  # else: refused below
-        rows, cols = _rows_cols(lx, normalized_dims)
+    lib = be.lib
+    if not hasattr(lib, "_wb_layers_declared"):
+        _declare(lib)
+    if 1 <= normalized_dims <= len(lx.shape) and (dt == DType.F32 or dt == DType.F64):  # else refused below
+        rows, cols = lx.rows_cols(normalized_dims)
         if out is None:
-            out = (be.alloc(lx.numel(), dt), be.alloc(cols, dt), be.alloc(cols, dt))
-        if workspace is None and cols and (out[1] is not None or out[2] is not None):
+            out = (be.alloc(rows * cols, dt), be.alloc(cols, dt), be.alloc(cols, dt))
+        dx, dweight, dbias = out
+        if workspace is None and cols and (dweight is not None or dbias is not None):
             workspace = layer_norm_workspace(be, rows, cols, dt)
-    dx, dweight, dbias = out if out is not None else (None, None, None)
-    size = 0 if workspace is None else workspace.length * DType.size(dt)
-    be.check(be.lib.wb_layer_norm_bwd(be.handle, vx, vg, normalized_dims, _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight),
-                                      _ptr(dbias), _ptr(workspace), size))
+        size = 4 if dt == DType.F32 else 8
+        wide, tall = cols * size, rows * size
+        if ((mean is not None and mean._bytes < tall) or (rstd is not None and rstd._bytes < tall) or (weight is not None and weight._bytes < wide)
+                or (dx is not None and dx._bytes < rows * wide) or (dweight is not None and dweight._bytes < wide)
+                or (dbias is not None and dbias._bytes < wide)):
+            _too_short("layer norm's gradients", dt, ("mean", mean, rows), ("rstd", rstd, rows), ("weight", weight, cols), ("dx", dx, rows * cols),
+                       ("dweight", dweight, cols), ("dbias", dbias, cols))
+    else:
+        dx, dweight, dbias = out if out is not None else (None, None, None)
+    status = lib.wb_layer_norm_bwd(be.handle, lx.view(x.ptr, dt), ldy.view(dy.ptr, dt), normalized_dims, None if weight is None else weight.ptr,
+                                   None if mean is None else mean.ptr, None if rstd is None else rstd.ptr, None if dx is None else dx.ptr, None if dweight is None else dweight.ptr,
+                                   None if dbias is None else dbias.ptr, None if workspace is None else workspace.ptr,
+                                   0 if workspace is None else workspace.nbytes)
+    if status:
+        be.check(status)
     return dx, dweight, dbias

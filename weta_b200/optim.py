@@ -53,6 +53,9 @@ class AdamMulti:
             raise BackendError(1, f"{len(no_decay)} no_decay flags for {n} tensors")
         self.params = list(params)
         lens = [p.length for p in params]
+        for i, p in enumerate(params):
+            if p.nbytes != 4 * p.length:
+                raise BackendError(1, f"parameter {i} is not f32")
         self.state_bytes = self.lib.wb_adam_multi_state_bytes((ctypes.c_int64 * max(n, 1))(*lens), n, state_bits)
         if state is None and self.state_bytes >= 0:
             if keep_state:
@@ -63,7 +66,7 @@ class AdamMulti:
                                            for i, (p, k) in enumerate(zip(params, lens))])
         out = ctypes.c_void_p()
         backend.check(self.lib.wb_adam_multi_create(backend.handle, arr, n, state_bits, None if state is None else state.ptr,
-                                                    0 if state is None else 4 * state.length, int(keep_state), ctypes.byref(out)))
+                                                    0 if state is None else state.nbytes, int(keep_state), ctypes.byref(out)))
         self.handle = out.value
         self.config = WbAdamConfig(lr, betas[0], betas[1], eps, weight_decay, int(decoupled))  # may be changed between steps
         self._config = ctypes.byref(self.config)
@@ -91,6 +94,8 @@ class AdamMulti:
         for i, (g, p) in enumerate(zip(grads, self.params)):
             if g is not None and g.length != p.length:
                 raise BackendError(1, f"gradient {i} has {g.length} elements, its parameter {p.length}")
+            if g is not None and g.nbytes != p.nbytes:
+                raise BackendError(1, f"gradient {i} is not f32")
         arr = (ctypes.c_void_p * max(len(grads), 1))(*[None if g is None else g.ptr for g in grads])
         self.be.check(self.lib.wb_adam_multi_set_grads(self.handle, arr, len(grads)))
         self._grads = list(grads)  # kept alive while the library holds their addresses
@@ -98,12 +103,16 @@ class AdamMulti:
     def grad_norm(self, max_norm: float, out: Optional[Sequence[DeviceStorage]] = None) -> Tuple[DeviceStorage, DeviceStorage]:
         """(norm of all gradients, min(1, max_norm / (norm + 1e-6))) as device scalars; the second is `step`'s grad_scale."""
         norm, scale = out if out is not None else (self.be.alloc(1, DType.F32), self.be.alloc(1, DType.F32))
+        if norm.nbytes < 4 or (scale is not None and scale.nbytes < 4):
+            raise BackendError(1, "an output of the norm holds no element")
         self.be.check(self.lib.wb_adam_multi_grad_norm(self.handle, max_norm, norm.ptr, None if scale is None else scale.ptr))
         return norm, scale
 
     def step(self, t: int, grad_scale: Union[None, float, DeviceStorage] = None):
         """Step t, counted from 1; the gradients are multiplied by `grad_scale`, a number or a device scalar."""
         if grad_scale is None or isinstance(grad_scale, DeviceStorage):
+            if grad_scale is not None and (grad_scale.length < 1 or grad_scale.nbytes != 4 * grad_scale.length):
+                raise BackendError(1, "the scale is not a storage of f32")
             host, device = 1.0, None if grad_scale is None else grad_scale.ptr
         else:
             host, device = float(grad_scale), None
@@ -112,5 +121,9 @@ class AdamMulti:
     def read_state(self, out: Optional[Sequence[Optional[DeviceStorage]]] = None) -> Tuple[DeviceStorage, DeviceStorage]:
         """(m, v) as f32 storages of `state_len` elements: what the state stands for."""
         m, v = out if out is not None else (self.be.alloc(self.state_len, DType.F32), self.be.alloc(self.state_len, DType.F32))
+        need = 4 * self.state_len
+        for s in (m, v):
+            if s is not None and s.nbytes < need:
+                raise BackendError(1, f"the moments take {need} bytes each, an output holds {s.nbytes}")
         self.be.check(self.lib.wb_adam_multi_read_state(self.handle, None if m is None else m.ptr, None if v is None else v.ptr))
         return m, v
