@@ -11,7 +11,9 @@ import numpy as np
 import pytest
 
 from weta_b200 import layers, optim
-from weta_b200.core import DType, Layout
+from weta_b200.backend import BackendError
+from weta_b200.core import BinaryOp, DType, Layout
+from weta_b200.fusion import FusingBackend
 from weta_b200.trainer import _declare
 
 pytestmark = pytest.mark.gpu
@@ -101,3 +103,53 @@ def test_training_steps(gpu, bits):
     finally:
         gpu.set_matmul_mode(0)
     gpu.gemm_check()
+
+
+def test_through_the_fusing_backend(gpu):
+    """Pending operands are evaluated, what reads a storage is evaluated before it is written over, and a pending value is no output."""
+    fb = FusingBackend(gpu)
+    rng = np.random.default_rng(3)
+    rows, cols = 6, 100
+    l, lc, one = Layout.contiguous([rows, cols]), Layout.contiguous([cols]), Layout.contiguous([1])
+    flat = Layout.contiguous([rows * cols])
+    x, dy = (rng.standard_normal(rows * cols).astype(np.float32) for _ in range(2))
+    w, b = (rng.standard_normal(cols).astype(np.float32) for _ in range(2))
+    down = lambda s, n: fb.to_host(s, Layout.contiguous([n]), DType.F32).copy()
+    keep = []
+
+    def twice(a, lay):
+        keep.append(gpu.from_host(a))
+        return fb.binary(BinaryOp.ADD, keep[-1], lay, keep[-1], lay, DType.F32)
+
+    want = layers.layer_norm_fwd(gpu, gpu.from_host(x + x), l, DType.F32, 1, gpu.from_host(w + w), gpu.from_host(b + b))
+    got = layers.layer_norm_fwd(fb, twice(x, l), l, DType.F32, 1, twice(w, lc), twice(b, lc))
+    for a, c, n in zip(got, want, (rows * cols, rows, rows)):
+        assert np.array_equal(down(a, n), down(c, n))
+    args = (l, DType.F32, 1)
+    wanted = layers.layer_norm_bwd(gpu, gpu.from_host(x + x), l, gpu.from_host(dy + dy), *args, gpu.from_host(w + w), *want[1:])
+    grads = layers.layer_norm_bwd(fb, twice(x, l), l, twice(dy, l), *args, twice(w, lc), *got[1:])
+    for a, c, n in zip(grads, wanted, (rows * cols, cols, cols)):
+        assert np.array_equal(down(a, n), down(c, n))
+
+    y = got[0]
+    old = down(y, rows * cols)
+    pending = fb.binary(BinaryOp.ADD, y, flat, y, flat, DType.F32)
+    layers.layer_norm_fwd(fb, gpu.from_host(dy), l, DType.F32, 1, out=got)
+    assert np.array_equal(down(pending, rows * cols), old + old) and not np.array_equal(down(y, rows * cols), old)
+    with pytest.raises(BackendError, match="can't be written over"):
+        layers.layer_norm_fwd(fb, gpu.from_host(dy), l, DType.F32, 1, out=(twice(x, l), None, None))
+
+    theta, other = gpu.from_host(x), gpu.from_host(x)
+    lazy, plain_ = optim.AdamMulti(fb, [theta], lr=0.1), optim.AdamMulti(gpu, [other], lr=0.1)
+    lazy.set_grads([twice(dy, flat)])
+    plain_.set_grads([gpu.from_host(dy + dy)])
+    pending = fb.binary(BinaryOp.ADD, theta, flat, theta, flat, DType.F32)
+    half = np.full(1, 0.25, np.float32)
+    lazy.step(1, twice(half, one))
+    plain_.step(1, gpu.from_host(half + half))
+    assert np.array_equal(down(pending, rows * cols), x + x)
+    assert np.array_equal(down(theta, rows * cols), down(other, rows * cols))
+    assert np.array_equal(down(lazy.grad_norm(1.0)[0], 1), down(plain_.grad_norm(1.0)[0], 1))
+    assert np.array_equal(down(lazy.read_state()[1], lazy.state_len), down(plain_.read_state()[1], lazy.state_len))
+    with pytest.raises(BackendError, match="can't be written over"):
+        optim.AdamMulti(fb, [twice(x, flat)])

@@ -161,7 +161,7 @@ class FakeLib:
 
 
 class FakeBackend:
-    lib, handle = FakeLib(), None
+    lib, handle, defers = FakeLib(), None, False
 
 
 def storage(n, dt=DType.F32):

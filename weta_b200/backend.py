@@ -134,6 +134,7 @@ class B200Backend:
     """One per GPU ordinal (crates/weta-cuda/src/lib.rs:129-146)."""
 
     name = "b200"
+    defers = False  # storages hold their values, and nothing pending reads them (see fusion.FusingBackend)
 
     def __init__(self, ordinal: int = 0, stream: Optional[int] = None):
         self.lib = load_library()

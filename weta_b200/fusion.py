@@ -18,7 +18,7 @@ import ctypes
 import weakref
 from typing import Dict, List, Optional, Tuple
 
-from .backend import B200Backend, DeviceStorage
+from .backend import B200Backend, BackendError, DeviceStorage
 from .core import DType, Layout, WbView
 
 MAX_INPUTS, MAX_INSTRS, MAX_OUTPUTS = 8, 48, 4
@@ -71,6 +71,7 @@ def _identity(layout: Layout, n: int) -> bool:
 
 class FusingBackend:
     name = "b200"
+    defers = True
 
     def __init__(self, inner: B200Backend):
         self.inner = inner
@@ -111,6 +112,20 @@ class FusingBackend:
 
     def _c(self, s):
         return s.concrete() if isinstance(s, LazyStorage) else s
+
+    # -- for calls that hand storages' addresses to the library themselves (layers.py, optim.py) ------------------
+    def for_reading(self, *storages):
+        """The storages with pending values evaluated; None stays."""
+        return tuple(self._c(s) for s in storages)
+
+    def for_writing(self, *storages):
+        """Evaluates what still has to read the storages' present contents; None stays."""
+        for s in storages:
+            if isinstance(s, LazyStorage):
+                raise BackendError(1, "the result of a deferred call can't be written over; give a storage of its own")
+            if s is not None:
+                self._flush_readers(s)
+        return storages
 
     # -- the lazy ops ----------------------------------------------------------------------
     def _source(self, s, layout: Layout):

@@ -47,6 +47,9 @@ def layer_norm_fwd(be: B200Backend, x: DeviceStorage, l: Layout, dt: int, normal
     lib = be.lib
     if not hasattr(lib, "_wb_layers_declared"):
         _declare(lib)
+    if be.defers:
+        x, weight, bias = be.for_reading(x, weight, bias)
+        out = None if out is None else be.for_writing(*out)
     if 1 <= normalized_dims <= len(l.shape) and (dt == DType.F32 or dt == DType.F64):
         rows, cols = l.rows_cols(normalized_dims)
         if out is None:
@@ -91,6 +94,10 @@ def layer_norm_bwd(be: B200Backend, x: DeviceStorage, lx: Layout, dy: DeviceStor
     lib = be.lib
     if not hasattr(lib, "_wb_layers_declared"):
         _declare(lib)
+    if be.defers:
+        x, dy, weight, mean, rstd = be.for_reading(x, dy, weight, mean, rstd)
+        out = None if out is None else be.for_writing(*out)
+        be.for_writing(workspace)
     if 1 <= normalized_dims <= len(lx.shape) and (dt == DType.F32 or dt == DType.F64):  # else refused below
         rows, cols = lx.rows_cols(normalized_dims)
         if out is None:

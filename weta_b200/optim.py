@@ -49,6 +49,8 @@ class AdamMulti:
         self.be, self.lib, self.handle = backend, backend.lib, None
         _declare(self.lib)
         n = len(params)
+        if backend.defers:
+            backend.for_writing(*params, state)
         if no_decay is not None and len(no_decay) != n:
             raise BackendError(1, f"{len(no_decay)} no_decay flags for {n} tensors")
         self.params = list(params)
@@ -91,6 +93,8 @@ class AdamMulti:
 
     def set_grads(self, grads: Sequence[Optional[DeviceStorage]]):
         """The gradients of the following calls, in the parameters' order; None leaves a tensor and its state alone."""
+        if self.be.defers:
+            grads = self.be.for_reading(*grads)
         for i, (g, p) in enumerate(zip(grads, self.params)):
             if g is not None and g.length != p.length:
                 raise BackendError(1, f"gradient {i} has {g.length} elements, its parameter {p.length}")
@@ -103,6 +107,8 @@ class AdamMulti:
     def grad_norm(self, max_norm: float, out: Optional[Sequence[DeviceStorage]] = None) -> Tuple[DeviceStorage, DeviceStorage]:
         """(norm of all gradients, min(1, max_norm / (norm + 1e-6))) as device scalars; the second is `step`'s grad_scale."""
         norm, scale = out if out is not None else (self.be.alloc(1, DType.F32), self.be.alloc(1, DType.F32))
+        if self.be.defers:
+            self.be.for_writing(norm, scale)
         if norm.nbytes < 4 or (scale is not None and scale.nbytes < 4):
             raise BackendError(1, "an output of the norm holds no element")
         self.be.check(self.lib.wb_adam_multi_grad_norm(self.handle, max_norm, norm.ptr, None if scale is None else scale.ptr))
@@ -110,6 +116,10 @@ class AdamMulti:
 
     def step(self, t: int, grad_scale: Union[None, float, DeviceStorage] = None):
         """Step t, counted from 1; the gradients are multiplied by `grad_scale`, a number or a device scalar."""
+        if self.be.defers:
+            self.be.for_writing(*self.params, self.state)
+            if hasattr(grad_scale, "ptr"):
+                grad_scale, = self.be.for_reading(grad_scale)
         if grad_scale is None or isinstance(grad_scale, DeviceStorage):
             if grad_scale is not None and (grad_scale.length < 1 or grad_scale.nbytes != 4 * grad_scale.length):
                 raise BackendError(1, "the scale is not a storage of f32")
@@ -121,6 +131,8 @@ class AdamMulti:
     def read_state(self, out: Optional[Sequence[Optional[DeviceStorage]]] = None) -> Tuple[DeviceStorage, DeviceStorage]:
         """(m, v) as f32 storages of `state_len` elements: what the state stands for."""
         m, v = out if out is not None else (self.be.alloc(self.state_len, DType.F32), self.be.alloc(self.state_len, DType.F32))
+        if self.be.defers:
+            self.be.for_writing(m, v)
         need = 4 * self.state_len
         for s in (m, v):
             if s is not None and s.nbytes < need:
