@@ -118,6 +118,18 @@ class FusingBackend:
         """The storages with pending values evaluated; None stays."""
         return tuple(self._c(s) for s in storages)
 
+    def for_keeping(self, *storages):
+        """As for_reading, where the addresses are used later: a value that shares the storage it was assigned to (see
+        copy_strided) gets one of its own, since that storage may be overwritten by then."""
+        for s in storages:
+            if isinstance(s, LazyStorage):
+                st, node = s.concrete(), s.node
+                sharing = self._aliases.get(st.handle)
+                if sharing is not None and node in sharing:
+                    node.concrete = self._copy_out(st, Layout.contiguous([node.n]), node.n)
+                    sharing.discard(node)
+        return self.for_reading(*storages)
+
     def for_writing(self, *storages):
         """Evaluates what still has to read the storages' present contents; None stays."""
         for s in storages:

@@ -94,7 +94,7 @@ class AdamMulti:
     def set_grads(self, grads: Sequence[Optional[DeviceStorage]]):
         """The gradients of the following calls, in the parameters' order; None leaves a tensor and its state alone."""
         if self.be.defers:
-            grads = self.be.for_reading(*grads)
+            grads = self.be.for_keeping(*grads)
         for i, (g, p) in enumerate(zip(grads, self.params)):
             if g is not None and g.length != p.length:
                 raise BackendError(1, f"gradient {i} has {g.length} elements, its parameter {p.length}")
