@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from host_backend import HostBackend
-from weta_b200 import optim
+from weta_b200 import layers, optim
 from weta_b200.core import BinaryOp, DType, Layout
 from weta_b200.fusion import FusingBackend
 
@@ -69,3 +69,27 @@ def test_a_gradient_given_as_a_storage_is_read_when_the_step_runs(fb):
     fb.copy_strided(g, L, DType.F32, buf, L)
     opt.step(1)
     assert np.array_equal(down(fb, theta), -2 * np.arange(N, dtype=F))
+
+
+def test_an_output_may_be_the_storage_that_an_operand_was_assigned_to(fb):
+    """The operand's value has a storage of its own in the plain backend, so the call is no overlap and reads the old value."""
+    rows = Layout.contiguous([1, N])
+    a, buf = up(fb, np.arange(N)), up(fb, np.zeros(N))
+    x = twice(fb, a)
+    fb.copy_strided(x, L, DType.F32, buf, L)
+    y, _, _ = layers.layer_norm_fwd(fb, x, rows, DType.F32, 1, out=(buf, None, None))
+    assert y is buf and np.array_equal(down(fb, x), 2 * np.arange(N, dtype=F))
+
+    dx, one = up(fb, np.zeros(N)), up(fb, np.zeros(1))
+    dy = twice(fb, a)
+    fb.copy_strided(dy, L, DType.F32, dx, L)
+    got, _, _ = layers.layer_norm_bwd(fb, a, rows, dy, rows, DType.F32, 1, None, one, one, out=(dx, None, None))
+    assert got is dx and np.array_equal(down(fb, dy), 2 * np.arange(N, dtype=F))
+
+    work = fb.inner.alloc(16, DType.F32)
+    l16 = Layout.contiguous([16])
+    w = twice(fb, fb.inner.from_host(np.ones(16, F)), l16)
+    fb.copy_strided(w, l16, DType.F32, work, l16)
+    s, g = up(fb, np.zeros(16)), up(fb, np.zeros(16))
+    layers.layer_norm_bwd(fb, s, Layout.contiguous([1, 16]), s, Layout.contiguous([1, 16]), DType.F32, 1, w, one, one, out=(None, g, None), workspace=work)
+    assert np.array_equal(fb.to_host(w, l16, DType.F32), np.full(16, 2, F))

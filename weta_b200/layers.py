@@ -47,9 +47,9 @@ def layer_norm_fwd(be: B200Backend, x: DeviceStorage, l: Layout, dt: int, normal
     lib = be.lib
     if not hasattr(lib, "_wb_layers_declared"):
         _declare(lib)
-    if be.defers:
-        x, weight, bias = be.for_reading(x, weight, bias)
+    if be.defers:  # the outputs first: an operand that shares the storage of one gets another storage there
         out = None if out is None else be.for_writing(*out)
+        x, weight, bias = be.for_reading(x, weight, bias)
     if 1 <= normalized_dims <= len(l.shape) and (dt == DType.F32 or dt == DType.F64):
         rows, cols = l.rows_cols(normalized_dims)
         if out is None:
@@ -94,10 +94,10 @@ def layer_norm_bwd(be: B200Backend, x: DeviceStorage, lx: Layout, dy: DeviceStor
     lib = be.lib
     if not hasattr(lib, "_wb_layers_declared"):
         _declare(lib)
-    if be.defers:
-        x, dy, weight, mean, rstd = be.for_reading(x, dy, weight, mean, rstd)
+    if be.defers:  # see layer_norm_fwd
         out = None if out is None else be.for_writing(*out)
         be.for_writing(workspace)
+        x, dy, weight, mean, rstd = be.for_reading(x, dy, weight, mean, rstd)
     if 1 <= normalized_dims <= len(lx.shape) and (dt == DType.F32 or dt == DType.F64):  # else refused below
         rows, cols = lx.rows_cols(normalized_dims)
         if out is None:
