@@ -93,3 +93,13 @@ def test_an_output_may_be_the_storage_that_an_operand_was_assigned_to(fb):
     s, g = up(fb, np.zeros(16)), up(fb, np.zeros(16))
     layers.layer_norm_bwd(fb, s, Layout.contiguous([1, 16]), s, Layout.contiguous([1, 16]), DType.F32, 1, w, one, one, out=(None, g, None), workspace=work)
     assert np.array_equal(fb.to_host(w, l16, DType.F32), np.full(16, 2, F))
+
+
+def test_nothing_of_a_closed_backend_is_used(fb):
+    """Closing the wrapped backend frees what the library keeps for the optimizer's handle: it is not destroyed after that."""
+    opt = optim.AdamMulti(fb, [up(fb, np.zeros(N))])
+    fb.inner.close()
+    assert not fb.handle
+    opt.close()
+    del opt
+    assert "destroy" not in fb.lib.calls

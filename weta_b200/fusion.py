@@ -76,7 +76,6 @@ class FusingBackend:
     def __init__(self, inner: B200Backend):
         self.inner = inner
         self.lib = inner.lib
-        self.handle = inner.handle
         self.ordinal = inner.ordinal
         P, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
         self.lib.wb_ew_fused.argtypes = [P, ctypes.POINTER(WbView), i32, ctypes.POINTER(WbEwInstr), i32, ctypes.POINTER(ctypes.c_int32),
@@ -89,6 +88,10 @@ class FusingBackend:
         self.ops_fused = 0     # trait calls those launches stood for (deferred calls never counted here were dropped unread)
 
     # -- plumbing shared with B200Backend ---------------------------------------------------
+    @property
+    def handle(self):  # None once the wrapped backend is closed
+        return self.inner.handle
+
     def check(self, status):
         self.inner.check(status)
 
