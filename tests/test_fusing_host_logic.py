@@ -4,6 +4,7 @@ import pytest
 
 from host_backend import HostBackend
 from weta_b200 import layers, optim
+from weta_b200.backend import BackendError
 from weta_b200.core import BinaryOp, DType, Layout
 from weta_b200.fusion import FusingBackend
 
@@ -103,3 +104,18 @@ def test_nothing_of_a_closed_backend_is_used(fb):
     opt.close()
     del opt
     assert "destroy" not in fb.lib.calls
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_an_optimizer_of_a_closed_backend_refuses(fused):
+    inner = HostBackend()
+    be = FusingBackend(inner) if fused else inner
+    theta, g, one, m = (inner.from_host(np.zeros(n, F)) for n in (N, N, 1, 256))
+    opt = optim.AdamMulti(be, [theta])
+    opt.set_grads([g])
+    inner.close()
+    for call in (lambda: opt.step(1), lambda: opt.step(1, one), lambda: opt.grad_norm(1.0), lambda: opt.grad_norm(1.0, out=(one, None)),
+                 opt.read_state, lambda: opt.read_state(out=(m, None))):
+        with pytest.raises(BackendError, match="backend is closed"):
+            call()
+    assert "step" not in inner.lib.calls and "read_state" not in inner.lib.calls

@@ -79,6 +79,18 @@ class AdamMulti:
             self.lib.wb_adam_multi_destroy(self.handle)
         self.handle = None
 
+    def _open(self):
+        if not self.be.handle:  # the library's handle points at the backend's memory
+            raise BackendError(1, "the optimizer's backend is closed")
+
+    def _call(self, entry, *args):
+        self._open()
+        self.be.check(entry(self.handle, *args))
+
+    def _alloc(self, n):
+        self._open()
+        return self.be.alloc(n, DType.F32)
+
     def __del__(self):
         if getattr(self, "handle", None):
             self.close()
@@ -106,17 +118,19 @@ class AdamMulti:
 
     def grad_norm(self, max_norm: float, out: Optional[Sequence[DeviceStorage]] = None) -> Tuple[DeviceStorage, DeviceStorage]:
         """(norm of all gradients, min(1, max_norm / (norm + 1e-6))) as device scalars; the second is `step`'s grad_scale."""
-        norm, scale = out if out is not None else (self.be.alloc(1, DType.F32), self.be.alloc(1, DType.F32))
+        norm, scale = out if out is not None else (self._alloc(1), self._alloc(1))
         if self.be.defers:
+            self._open()
             self.be.for_writing(norm, scale)
         if norm.nbytes < 4 or (scale is not None and scale.nbytes < 4):
             raise BackendError(1, "an output of the norm holds no element")
-        self.be.check(self.lib.wb_adam_multi_grad_norm(self.handle, max_norm, norm.ptr, None if scale is None else scale.ptr))
+        self._call(self.lib.wb_adam_multi_grad_norm, max_norm, norm.ptr, None if scale is None else scale.ptr)
         return norm, scale
 
     def step(self, t: int, grad_scale: Union[None, float, DeviceStorage] = None):
         """Step t, counted from 1; the gradients are multiplied by `grad_scale`, a number or a device scalar."""
         if self.be.defers:
+            self._open()
             self.be.for_writing(*self.params, self.state)
             if hasattr(grad_scale, "ptr"):
                 grad_scale, = self.be.for_reading(grad_scale)
@@ -126,16 +140,17 @@ class AdamMulti:
             host, device = 1.0, None if grad_scale is None else grad_scale.ptr
         else:
             host, device = float(grad_scale), None
-        self.be.check(self.lib.wb_adam_multi_step(self.handle, self._config, t, host, device))
+        self._call(self.lib.wb_adam_multi_step, self._config, t, host, device)
 
     def read_state(self, out: Optional[Sequence[Optional[DeviceStorage]]] = None) -> Tuple[DeviceStorage, DeviceStorage]:
         """(m, v) as f32 storages of `state_len` elements: what the state stands for."""
-        m, v = out if out is not None else (self.be.alloc(self.state_len, DType.F32), self.be.alloc(self.state_len, DType.F32))
+        m, v = out if out is not None else (self._alloc(self.state_len), self._alloc(self.state_len))
         if self.be.defers:
+            self._open()
             self.be.for_writing(m, v)
         need = 4 * self.state_len
         for s in (m, v):
             if s is not None and s.nbytes < need:
                 raise BackendError(1, f"the moments take {need} bytes each, an output holds {s.nbytes}")
-        self.be.check(self.lib.wb_adam_multi_read_state(self.handle, None if m is None else m.ptr, None if v is None else v.ptr))
+        self._call(self.lib.wb_adam_multi_read_state, None if m is None else m.ptr, None if v is None else v.ptr)
         return m, v
