@@ -107,9 +107,14 @@ class DeviceStorage:
     def __init__(self, handle: int, backend: "B200Backend"):
         self.handle = handle
         self.backend = backend
-        self.ptr = backend.lib.wb_storage_data(handle)  # neither address nor length changes while the handle lives
-        self._length = None
-        self._bytes = 0  # not asked for yet
+        self._length = None  # not asked for yet, and neither are the bytes and the address: most results are never asked
+        self._bytes = 0
+
+    def __getattr__(self, name):  # the address, when it is first read; it does not change while the handle lives
+        if name != "ptr":
+            raise AttributeError(f"DeviceStorage has no attribute {name!r}")
+        self.ptr = self.backend.lib.wb_storage_data(self.handle)
+        return self.ptr
 
     @property
     def length(self) -> int:
