@@ -1,0 +1,50 @@
+"""CPU-only: layer norm and the many-tensor optimizer refuse storages of another element type, however long they are."""
+import pytest
+
+from weta_b200 import layers
+from weta_b200.backend import BackendError, DeviceStorage
+from weta_b200.core import DType, Layout
+
+
+class NoLib:
+    """Fails the test where a call gets as far as the library."""
+    _wb_layers_declared = _wb_optim_declared = True
+
+    def __getattr__(self, name):
+        raise AssertionError(f"{name} was called")
+
+
+class NoBackend:
+    defers, handle = False, None
+
+    def __init__(self, dt=DType.F32, n=1 << 20):
+        self.lib = NoLib()
+        self.lib.wb_storage_dtype = lambda handle: dt
+        self.lib.wb_storage_len = lambda handle: n
+        self.lib.wb_storage_data = lambda handle: 1 << 32
+
+
+def storage(dt, n=1 << 20):
+    return DeviceStorage(0, NoBackend(dt, n))
+
+
+NAMES = {DType.F32: "f32", DType.F64: "f64", DType.I64: "i64"}
+OTHERS = [(DType.F32, DType.F64), (DType.F32, DType.I64), (DType.F64, DType.F32), (DType.F64, DType.I64)]
+
+
+@pytest.mark.parametrize("dt,other", OTHERS)
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "y", "mean", "rstd"])
+def test_forward(which, dt, other):
+    s = {k: storage(other if k == which else dt) for k in ("x", "weight", "bias", "y", "mean", "rstd")}
+    with pytest.raises(BackendError, match=f"{which} is of {NAMES[other]}, not {NAMES[dt]}"):
+        layers.layer_norm_fwd(NoBackend(), s["x"], Layout.contiguous([4, 8]), dt, 1, s["weight"], s["bias"], out=(s["y"], s["mean"], s["rstd"]))
+
+
+@pytest.mark.parametrize("dt,other", OTHERS)
+@pytest.mark.parametrize("which", ["x", "dy", "weight", "mean", "rstd", "dx", "dweight", "dbias"])
+def test_backward(which, dt, other):
+    s = {k: storage(other if k == which else dt) for k in ("x", "dy", "weight", "mean", "rstd", "dx", "dweight", "dbias")}
+    l = Layout.contiguous([4, 8])
+    with pytest.raises(BackendError, match=f"{which} is of {NAMES[other]}, not {NAMES[dt]}"):
+        layers.layer_norm_bwd(NoBackend(), s["x"], l, s["dy"], l, dt, 1, s["weight"], s["mean"], s["rstd"], out=(s["dx"], s["dweight"], s["dbias"]),
+                              workspace=storage(dt))

@@ -102,19 +102,22 @@ def load_library():
 class DeviceStorage:
     """An owned WbStorage handle; returns its block to the backend's arena when collected."""
 
-    __slots__ = ("handle", "backend", "ptr", "_length", "_bytes", "__weakref__")
+    __slots__ = ("handle", "backend", "ptr", "dtype", "_length", "_bytes", "__weakref__")
 
     def __init__(self, handle: int, backend: "B200Backend"):
         self.handle = handle
         self.backend = backend
-        self._length = None  # not asked for yet, and neither are the bytes and the address: most results are never asked
+        self._length = None  # not asked for yet, and neither are the bytes, the address and the type: most results never are
         self._bytes = 0
 
-    def __getattr__(self, name):  # the address, when it is first read; it does not change while the handle lives
-        if name != "ptr":
-            raise AttributeError(f"DeviceStorage has no attribute {name!r}")
-        self.ptr = self.backend.lib.wb_storage_data(self.handle)
-        return self.ptr
+    def __getattr__(self, name):  # the address and the type, when first read; they do not change while the handle lives
+        if name == "ptr":
+            self.ptr = self.backend.lib.wb_storage_data(self.handle)
+            return self.ptr
+        if name == "dtype":
+            self.dtype = self.backend.lib.wb_storage_dtype(self.handle)
+            return self.dtype
+        raise AttributeError(f"DeviceStorage has no attribute {name!r}")
 
     @property
     def length(self) -> int:
@@ -125,7 +128,7 @@ class DeviceStorage:
     @property
     def nbytes(self) -> int:
         if self._bytes == 0:
-            self._bytes = self.length * DType.size(self.backend.lib.wb_storage_dtype(self.handle))
+            self._bytes = self.length * DType.size(self.dtype)
         return self._bytes
 
     def __del__(self):
@@ -196,7 +199,9 @@ class B200Backend:
     def alloc(self, n: int, dt: int) -> DeviceStorage:
         out = ctypes.c_void_p()
         self.check(self.lib.wb_alloc(self.handle, n, dt, ctypes.byref(out)))
-        return self._wrap(out)
+        s = self._wrap(out)
+        s._length, s.dtype, s._bytes = n, dt, n * DType.size(dt)
+        return s
 
     def wrap_pointer(self, ptr: int, n: int, dt: int) -> DeviceStorage:
         out = ctypes.c_void_p()

@@ -1,8 +1,8 @@
 """Fused layer ops on device storages: layer normalisation, forward and backward (include/weta_b200.h `wb_layer_norm_*`).
 
 Tensors come as (storage, Layout, dtype), the way the backend's own methods take them; results are fresh contiguous
-storages from the backend's arena unless `out` gives them.  Storages that are taken whole are checked for their length; a
-view is not checked against its storage, as in the backend's methods.
+storages from the backend's arena unless `out` gives them.  All storages are checked for their element type, and those that
+are taken whole for their length; a view is not checked against its storage, as in the backend's methods.
 """
 from __future__ import annotations
 
@@ -30,11 +30,13 @@ def _declare(lib):
     lib._wb_layers_declared = True
 
 
-def _too_short(what: str, dt: int, *needs: Tuple[str, Optional[DeviceStorage], int]):
-    """Refuses storages that hold fewer than so many elements of dtype `dt`."""
+def _check(what: str, dt: int, *needs: Tuple[str, Optional[DeviceStorage], int]):
+    """Refuses storages that hold fewer than so many elements of dtype `dt`, or elements of another type."""
     for name, s, n in needs:
         if s is not None and s.nbytes < n * DType.size(dt):
             raise BackendError(_INVALID, f"{what}: {name} holds {s.nbytes} bytes, {n * DType.size(dt)} are needed")
+        if s is not None and s.dtype != dt:
+            raise BackendError(_INVALID, f"{what}: {name} is of {DType.name(s.dtype)}, not {DType.name(dt)}")
 
 
 def layer_norm_fwd(be: B200Backend, x: DeviceStorage, l: Layout, dt: int, normalized_dims: int, weight: Optional[DeviceStorage] = None,
@@ -56,12 +58,14 @@ def layer_norm_fwd(be: B200Backend, x: DeviceStorage, l: Layout, dt: int, normal
             out = (be.alloc(rows * cols, dt), be.alloc(rows, dt), be.alloc(rows, dt))
         y, mean, rstd = out
         size = 4 if dt == DType.F32 else 8
-        # the lengths in bytes as far as they are known: those that are not read as 0, and _too_short asks for them
-        if ((weight is not None and weight._bytes < cols * size) or (bias is not None and bias._bytes < cols * size)
-                or (y is not None and y._bytes < rows * cols * size) or (mean is not None and mean._bytes < rows * size)
-                or (rstd is not None and rstd._bytes < rows * size)):
-            _too_short("layer norm", dt, ("weight", weight, cols), ("bias", bias, cols), ("y", y, rows * cols), ("mean", mean, rows),
-                       ("rstd", rstd, rows))
+        # the lengths in bytes as far as they are known: those that are not read as 0, and _check asks for them
+        if (x.dtype != dt or (weight is not None and (weight._bytes < cols * size or weight.dtype != dt))
+                or (bias is not None and (bias._bytes < cols * size or bias.dtype != dt))
+                or (y is not None and (y._bytes < rows * cols * size or y.dtype != dt))
+                or (mean is not None and (mean._bytes < rows * size or mean.dtype != dt))
+                or (rstd is not None and (rstd._bytes < rows * size or rstd.dtype != dt))):
+            _check("layer norm", dt, ("x", x, 0), ("weight", weight, cols), ("bias", bias, cols), ("y", y, rows * cols), ("mean", mean, rows),
+                   ("rstd", rstd, rows))
     else:  # refused below, with the library's message
         y, mean, rstd = x, None, None
     status = lib.wb_layer_norm_fwd(be.handle, l.view(x.ptr, dt), normalized_dims, None if weight is None else weight.ptr,
@@ -107,11 +111,14 @@ def layer_norm_bwd(be: B200Backend, x: DeviceStorage, lx: Layout, dy: DeviceStor
             workspace = layer_norm_workspace(be, rows, cols, dt)
         size = 4 if dt == DType.F32 else 8
         wide, tall = cols * size, rows * size
-        if ((mean is not None and mean._bytes < tall) or (rstd is not None and rstd._bytes < tall) or (weight is not None and weight._bytes < wide)
-                or (dx is not None and dx._bytes < rows * wide) or (dweight is not None and dweight._bytes < wide)
-                or (dbias is not None and dbias._bytes < wide)):
-            _too_short("layer norm's gradients", dt, ("mean", mean, rows), ("rstd", rstd, rows), ("weight", weight, cols), ("dx", dx, rows * cols),
-                       ("dweight", dweight, cols), ("dbias", dbias, cols))
+        if (x.dtype != dt or dy.dtype != dt or (mean is not None and (mean._bytes < tall or mean.dtype != dt))
+                or (rstd is not None and (rstd._bytes < tall or rstd.dtype != dt))
+                or (weight is not None and (weight._bytes < wide or weight.dtype != dt))
+                or (dx is not None and (dx._bytes < rows * wide or dx.dtype != dt))
+                or (dweight is not None and (dweight._bytes < wide or dweight.dtype != dt))
+                or (dbias is not None and (dbias._bytes < wide or dbias.dtype != dt))):
+            _check("layer norm's gradients", dt, ("x", x, 0), ("dy", dy, 0), ("mean", mean, rows), ("rstd", rstd, rows), ("weight", weight, cols),
+                   ("dx", dx, rows * cols), ("dweight", dweight, cols), ("dbias", dbias, cols))
     else:
         dx, dweight, dbias = out if out is not None else (None, None, None)
     status = lib.wb_layer_norm_bwd(be.handle, lx.view(x.ptr, dt), ldy.view(dy.ptr, dt), normalized_dims, None if weight is None else weight.ptr,
