@@ -1,7 +1,7 @@
 """CPU-only: layer norm and the many-tensor optimizer refuse storages of another element type, however long they are."""
 import pytest
 
-from weta_b200 import layers
+from weta_b200 import layers, optim
 from weta_b200.backend import BackendError, DeviceStorage
 from weta_b200.core import DType, Layout
 
@@ -48,3 +48,40 @@ def test_backward(which, dt, other):
     with pytest.raises(BackendError, match=f"{which} is of {NAMES[other]}, not {NAMES[dt]}"):
         layers.layer_norm_bwd(NoBackend(), s["x"], l, s["dy"], l, dt, 1, s["weight"], s["mean"], s["rstd"], out=(s["dx"], s["dweight"], s["dbias"]),
                               workspace=storage(dt))
+
+
+def optimizer():
+    o = optim.AdamMulti.__new__(optim.AdamMulti)
+    o.be, o.lib, o.handle, o.params = NoBackend(), NoLib(), None, [storage(DType.F32, 10)]
+    o.be.handle = 1
+    o.lib.wb_adam_multi_state_len = lambda handle: 256
+    return o
+
+
+@pytest.mark.parametrize("other", [DType.F64, DType.I64])
+@pytest.mark.parametrize("which", [0, 1])
+def test_scalars_of_the_norm(which, other):
+    out = [storage(DType.F32), storage(DType.F32)]
+    out[which] = storage(other)
+    with pytest.raises(BackendError, match=f"{('norm', 'clip factor')[which]} is of {NAMES[other]}, not f32"):
+        optimizer().grad_norm(1.0, out=out)
+
+
+@pytest.mark.parametrize("other", [DType.F64, DType.I64])
+@pytest.mark.parametrize("which", [0, 1])
+def test_moments_that_are_read_back(which, other):
+    for rest in (storage(DType.F32), None):
+        out = [rest, rest]
+        out[which] = storage(other)
+        with pytest.raises(BackendError, match=f"{'mv'[which]} is of {NAMES[other]}, not f32"):
+            optimizer().read_state(out=out)
+
+
+@pytest.mark.parametrize("other", [DType.F64, DType.I64])
+def test_parameters_gradients_and_the_scale(other):
+    with pytest.raises(BackendError, match="parameter 0 is not f32"):
+        optim.AdamMulti(NoBackend(), [storage(other, 10)])
+    with pytest.raises(BackendError, match="gradient 0 is not f32"):
+        optimizer().set_grads([storage(other, 10)])
+    with pytest.raises(BackendError, match="scale is not a storage of f32"):
+        optimizer().step(1, storage(other, 1))

@@ -34,6 +34,11 @@ def _declare(lib):
     lib._wb_optim_declared = True
 
 
+def _check_f32(name: str, s: Optional[DeviceStorage]):
+    if s is not None and s.dtype != DType.F32:
+        raise BackendError(1, f"{name} is of {DType.name(s.dtype)}, not f32")
+
+
 class AdamMulti:
     """The optimizer of a list of f32 parameter storages (crates/weta-optim/src/lib.rs:178-239, 276-283).
 
@@ -56,7 +61,7 @@ class AdamMulti:
         self.params = list(params)
         lens = [p.length for p in params]
         for i, p in enumerate(params):
-            if p.nbytes != 4 * p.length:
+            if p.dtype != DType.F32:
                 raise BackendError(1, f"parameter {i} is not f32")
         self.state_bytes = self.lib.wb_adam_multi_state_bytes((ctypes.c_int64 * max(n, 1))(*lens), n, state_bits)
         if state is None and self.state_bytes >= 0:
@@ -110,7 +115,7 @@ class AdamMulti:
         for i, (g, p) in enumerate(zip(grads, self.params)):
             if g is not None and g.length != p.length:
                 raise BackendError(1, f"gradient {i} has {g.length} elements, its parameter {p.length}")
-            if g is not None and g.nbytes != p.nbytes:
+            if g is not None and g.dtype != DType.F32:
                 raise BackendError(1, f"gradient {i} is not f32")
         arr = (ctypes.c_void_p * max(len(grads), 1))(*[None if g is None else g.ptr for g in grads])
         self.be.check(self.lib.wb_adam_multi_set_grads(self.handle, arr, len(grads)))
@@ -124,6 +129,8 @@ class AdamMulti:
             self.be.for_writing(norm, scale)
         if norm.nbytes < 4 or (scale is not None and scale.nbytes < 4):
             raise BackendError(1, "an output of the norm holds no element")
+        _check_f32("the norm", norm)
+        _check_f32("the clip factor", scale)
         self._call(self.lib.wb_adam_multi_grad_norm, max_norm, norm.ptr, None if scale is None else scale.ptr)
         return norm, scale
 
@@ -135,7 +142,7 @@ class AdamMulti:
             if hasattr(grad_scale, "ptr"):
                 grad_scale, = self.be.for_reading(grad_scale)
         if grad_scale is None or isinstance(grad_scale, DeviceStorage):
-            if grad_scale is not None and (grad_scale.length < 1 or grad_scale.nbytes != 4 * grad_scale.length):
+            if grad_scale is not None and (grad_scale.length < 1 or grad_scale.dtype != DType.F32):
                 raise BackendError(1, "the scale is not a storage of f32")
             host, device = 1.0, None if grad_scale is None else grad_scale.ptr
         else:
@@ -149,8 +156,9 @@ class AdamMulti:
             self._open()
             self.be.for_writing(m, v)
         need = 4 * self.state_len
-        for s in (m, v):
+        for name, s in (("m", m), ("v", v)):
             if s is not None and s.nbytes < need:
                 raise BackendError(1, f"the moments take {need} bytes each, an output holds {s.nbytes}")
+            _check_f32(name, s)
         self._call(self.lib.wb_adam_multi_read_state, None if m is None else m.ptr, None if v is None else v.ptr)
         return m, v
