@@ -138,6 +138,9 @@ class Layout:
         self.offset = int(offset)
         self._view = self._rows = None
 
+    def __reduce__(self):  # a copy or a pickle takes what makes the layout, not what is kept for its calls
+        return type(self), (self.shape, self.strides, self.offset)
+
     @staticmethod
     def contiguous(shape: Sequence[int]) -> "Layout":
         return Layout(shape, contiguous_strides(shape), 0)
@@ -152,10 +155,10 @@ class Layout:
     def rows_cols(self, inner_dims: int) -> Tuple[int, int]:
         """The elements of the dims before the last `inner_dims`, and of those."""
         r = self._rows
-        if r is None or r[0] != inner_dims:
+        if r is None or r[0] != inner_dims or r[1] != self.shape:
             outer = self.ndim - inner_dims
-            r = self._rows = (inner_dims, (math.prod(self.shape[:outer]), math.prod(self.shape[outer:])))
-        return r[1]
+            r = self._rows = (inner_dims, tuple(self.shape), (math.prod(self.shape[:outer]), math.prod(self.shape[outer:])))
+        return r[2]
 
     def is_contiguous(self) -> bool:  # layout.rs:60-69
         expected = 1
@@ -226,11 +229,13 @@ class Layout:
 
     def view(self, data: int, dtype: int) -> WbView:
         form = self._view
-        if form is None:  # what does not depend on the storage; filling the arrays costs ten times a copy of the whole
+        # what does not depend on the storage is kept, with the values it was made from: filling the arrays costs ten times a
+        # copy of the whole
+        if form is None or form[0] != self.shape or form[1] != self.strides or form[2] != self.offset:
             assert self.ndim <= MAX_DIMS, f"at most {MAX_DIMS} dims are supported, got shape {self.shape}"
-            rest = MAX_DIMS - self.ndim
-            form = self._view = WbView(None, 0, self.ndim, self.shape + (1,) * rest, self.strides + (0,) * rest, self.offset)
-        v = WbView.from_buffer_copy(form)
+            shape, strides, rest = tuple(self.shape), tuple(self.strides), MAX_DIMS - self.ndim
+            form = self._view = (shape, strides, self.offset, WbView(None, 0, self.ndim, shape + (1,) * rest, strides + (0,) * rest, self.offset))
+        v = WbView.from_buffer_copy(form[3])
         v.data = data
         v.dtype = dtype
         return v
