@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from weta_b200 import optim
+from weta_b200 import layers, optim
 from weta_b200.core import BinaryOp, DType, Layout
 from weta_b200.fusion import FusingBackend
 
@@ -39,3 +39,35 @@ def test_a_deferred_gradient_assigned_to_a_storage_that_changes(gpu, dropped):
     for p, q in zip(*results):
         assert np.array_equal(p, q)
     assert np.array_equal(results[0][2], other)
+
+
+BIG = {DType.F32: 1e36, DType.F64: 1e306}
+
+
+@pytest.mark.parametrize("cols", [3, 21, 36, 64, 131, 200, 256, 257, 520, 777, 1024, 1544, 3080, 4100, 5001, 8192, 9000, 9001, 17000])
+@pytest.mark.parametrize("dt", [DType.F32, DType.F64])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_rows_of_one_huge_value_have_a_finite_gradient(gpu, cols, dt, shift):
+    """xhat is 0 in such a row however large the value, and dx = rstd (g - mean g); the statistics are given, since the forward
+    pass's sum of that many such values may overflow.  The widths fill a thread's last vector and leave it partly empty.
+    Tolerance as for every row: 60 u rstd (|g| + mean |g|), and u |xhat| terms that are 0 here."""
+    rng = np.random.default_rng(cols + shift)
+    rows, rstd = 5, 1024.0
+    u, t = U[dt], NP[dt]
+    x = rng.standard_normal((rows, cols)).astype(t)
+    mean = x.mean(1).astype(t)
+    for k, v in ((1, BIG[dt]), (3, -BIG[dt]), (4, 2.0)):
+        x[k] = mean[k] = v
+    dy, w = rng.standard_normal((rows, cols)).astype(t), rng.uniform(0.5, 1.5, cols).astype(t)
+    l = Layout.contiguous([rows, cols])
+    sg = gpu.from_host(np.concatenate([np.zeros(shift, t), dy.reshape(-1)]))
+    out = layers.layer_norm_bwd(gpu, gpu.from_host(x.reshape(-1)), l, sg, Layout([rows, cols], [cols, 1], shift), dt, 1, gpu.from_host(w),
+                                gpu.from_host(mean), gpu.from_host(np.full(rows, rstd, t)))
+    dx, dw, db = (down(gpu, s, n, dt) for s, n in zip(out, (rows * cols, cols, cols)))
+    g = dy.astype(np.longdouble) * w
+    xh = (x.astype(np.longdouble) - mean.astype(np.longdouble)[:, None]) * rstd
+    s, p = g.mean(1, keepdims=True), (g * xh).mean(1, keepdims=True)
+    bound = 60 * u * rstd * (np.abs(g) + np.abs(g).mean(1, keepdims=True) + np.abs(xh) * np.abs(g * xh).mean(1, keepdims=True))
+    assert (np.abs(dx.reshape(rows, cols) - rstd * (g - s - xh * p)) <= bound).all()
+    assert (np.abs(dw - (dy * xh).sum(0)) <= (16 + rows) * u * np.abs(dy * xh).sum(0)).all()
+    assert (np.abs(db - dy.sum(0, dtype=np.longdouble)) <= (16 + rows) * u * np.abs(dy).sum(0)).all()

@@ -377,6 +377,11 @@ __device__ __forceinline__ void replace_outside(int c, int cols, const T& with, 
     }
 }
 
+// Whether (0 - mean) rstd is not finite.  Places that are not of a row hold zeros in the backward pass (MIXED: the row's mean);
+// their weight is zero, but zero times an infinity is not: in such a row (equal values of 2e36, say) they are left out.
+__device__ __forceinline__ bool far_from_zero(float mean, float rstd) { return !(fabsf(mean * rstd) <= 3.402823466e38f); }
+__device__ __forceinline__ bool far_from_zero(double mean, double rstd) { return !(fabs(mean * rstd) <= 1.7976931348623157e308); }
+
 constexpr int SPAN_THREADS = 512;
 constexpr int MOST_SHARED = 216 << 10;
 
@@ -588,6 +593,18 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
             }
             if (!dx) continue;
             T s[2], lo, hi;
+            if (MODE != MIXED && far_from_zero(mu, rs)) {
+                s1 = pair(T(0), T(0));
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int i = 0; i < H; ++i) {
+                        const int c = column(j, 2 * i), d = column(j, 2 * i + 1);
+                        unpair(xh[j][i], lo, hi);
+                        const Pair<T> x2 = pair(c >= 0 && c < sh.cols ? lo : T(0), d >= 0 && d < sh.cols ? hi : T(0));
+                        if (live) s1 = muladd(gv[j][i], x2, s1);
+                    }
+            }
             unpair(s0, lo, hi);
             s[0] = lo + hi;
             unpair(s1, lo, hi);
@@ -782,11 +799,13 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
             bar_wait(&full[slot], phase, limit);
             const T mu = ring[slot * slot_elems + 2 * sh.cap - U], rs = ring[slot * slot_elems + 2 * sh.cap - U + 32];
             const Pair<T> minus_mu = pair(-mu, -mu), rs2 = pair(rs, rs);
+            const bool far = far_from_zero(mu, rs);
             Pair<T> s0 = pair(T(0), T(0)), s1 = s0;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 Pair<T> xh[H], up[H];
                 load(row, slot, j, mu, minus_mu, rs2, xh, up);
+                if (MODE != MIXED && far) replace_outside(col.first(j), to, T(0), xh);
 #pragma unroll
                 for (int i = 0; i < H; ++i) {
                     const Pair<T> gv = up[i] * wv[j][i];
