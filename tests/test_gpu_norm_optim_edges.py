@@ -71,3 +71,45 @@ def test_rows_of_one_huge_value_have_a_finite_gradient(gpu, cols, dt, shift):
     assert (np.abs(dx.reshape(rows, cols) - rstd * (g - s - xh * p)) <= bound).all()
     assert (np.abs(dw - (dy * xh).sum(0)) <= (16 + rows) * u * np.abs(dy * xh).sum(0)).all()
     assert (np.abs(db - dy.sum(0, dtype=np.longdouble)) <= (16 + rows) * u * np.abs(dy).sum(0)).all()
+
+
+@pytest.mark.parametrize("eps,lr,scale", [(2.0 ** 100, 2.0 ** 110, 2.0 ** -26), (2.0 ** 90, 2.0 ** 100, 2.0 ** -40), (2.0 ** 60, 2.0 ** 70, 2.0 ** -55),
+                                          (2.0 ** 66, 2.0 ** 80, 1.0), (1e-8, 1.0, 2.0 ** 41), (1e-8, 1.0, 2.0 ** 58)])
+def test_8_bit_step_with_quotients_near_and_below_the_normal_range(gpu, eps, lr, scale):
+    """m / (root + eps) rounded once, subnormal or not: theta starts at 0, so its first value is that quotient times lr.  Gradients
+    lie within a factor of 8, and beta2 near 1 makes 1 / sqrt(1 - beta2^t) as large as 2^13."""
+    from test_gpu_adam_multi import Plain, same
+
+    n, b2 = 256 * 64, 1 - 2.0 ** -26
+    rng = np.random.default_rng(2)
+    g = (rng.uniform(1, 8, n) * rng.choice([-1, 1], n) * scale).astype(F)
+    th = np.zeros(n, F)
+    store = gpu.from_host(th)
+    opt = optim.AdamMulti(gpu, [store], 8, lr=lr, betas=(0.9, b2), eps=eps)
+    opt.set_grads([gpu.from_host(g)])
+    p = Plain(n, 8)
+    with np.errstate(all="ignore"):
+        for t in (1, 2):
+            opt.step(t)
+            th = p.step(th, g, t, lr, 0.9, b2, eps, 0.0, False, False, None)
+            assert np.abs(th).max() > 0 and same(down(gpu, store, n), th), t
+
+
+@pytest.mark.parametrize("c", [3, 5, 7, 11, 13])
+def test_8_bit_step_with_subnormal_quotients_half_way_between_two(gpu, c):
+    """With both betas 0 the first step is theta - g / (|g| + eps) lr, and |g| + eps rounds to eps = c 2^98.  g = c (2k + 1) 2^-52
+    makes the quotient (2k + 1) 2^-150, half way between two subnormal values: it goes to the even one."""
+    from test_gpu_adam_multi import Plain, same
+
+    n, eps, lr = 256 * 64, c * 2.0 ** 98, 2.0 ** 120
+    k = np.arange(8, n + 8)
+    g = (c * (2 * k + 1) * 2.0 ** -52).astype(F)
+    assert (g.astype(np.float64) == c * (2 * k + 1) * 2.0 ** -52).all()
+    store = gpu.zeros(n, DType.F32)
+    opt = optim.AdamMulti(gpu, [store], 8, lr=lr, betas=(0.0, 0.0), eps=eps)
+    opt.set_grads([gpu.from_host(g)])
+    opt.step(1)
+    even = (k + (k & 1)) * 2.0 ** (120 - 149)
+    got = down(gpu, store, n)
+    assert np.array_equal(got, -even.astype(F))
+    assert same(got, Plain(n, 8).step(np.zeros(n, F), g, 1, lr, 0.0, 0.0, eps, 0.0, False, False, None))

@@ -239,7 +239,7 @@ struct AdamK8 {
     float gscale, decay_mul;  // 1 where there is none: x * 1 is x
     float wd, inv_sqrt_bc2, eps, step;
     int l2;          // weight decay through the gradient
-    int eps_normal;  // eps is at least 2^-60
+    int eps_normal;  // eps is in [2^-60, 2^60] and inv_sqrt_bc2 at most 2^20
 };
 
 // One warp takes a block of 256 elements, a lane the groups of four at 4 lane and 128 + 4 lane.
@@ -338,9 +338,10 @@ __global__ void __launch_bounds__(THREADS, 5) adam_multi8_kernel(const __grid_co
         top_v = largest_or_nan(top_v, a, b);
         low_v = least(low_v, a, b);
     }
-    // m in [2^-60, 2^60], v in [2^-100, 2^120] and eps at least 2^-60: nothing below leaves the normal range
+    // m in [2^-60, 2^60], v in [2^-100, 2^80], eps in [2^-60, 2^60] and 1 / sqrt(1 - beta2^t) at most 2^20: the denominator lies in
+    // [2^-60, 2^61] and the quotient in [2^-121, 2^120], so nothing leaves the normal range before the quotient is multiplied
     if (k8.eps_normal && low_m >= 8.6736173798840355e-19f && low_v >= 7.8886090522101181e-31f && top_m <= 1.152921504606847e18f &&
-        top_v <= 1.3292279957849159e36f) {
+        top_v <= 1.2089258196146292e24f) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             root[j] = root_of(root[j]);
@@ -761,7 +762,7 @@ extern "C" int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64
     k8.inv_sqrt_bc2 = k.inv_sqrt_bc2;
     k8.eps = k.eps;
     k8.step = k.step_size;
-    k8.eps_normal = k.eps >= 8.6736173798840355e-19f && k.inv_sqrt_bc2 <= 1048576.f;
+    k8.eps_normal = k.eps >= 8.6736173798840355e-19f && k.eps <= 1.152921504606847e18f && k.inv_sqrt_bc2 <= 1048576.f;
     k8.minus_step = twice(-k.step_size);
     k8.minus_zero = twice(-0.f);
     k8.gscale = k.scale_grad ? k.gscale : 1.f;
