@@ -184,13 +184,15 @@ double wb_host_normal_sample(uint64_t seed, uint64_t i, double mean, double std)
 
 /* ==== extension: entry points with no trait method today ===================================== */
 
-/* Reads the device-side flag a tensor-core kernel (or the layer norm's) raises when one of its bounded barrier waits
- * runs out (WB_ERR_TIMEOUT), then clears it.  Synchronises the stream.  The reference has no
+/* Reads the flags that this backend's tensor-core kernels and layer norms raise when one of their bounded barrier waits
+ * runs out (WB_ERR_TIMEOUT), then clears them.  Synchronises the stream.  The reference has no
  * counterpart: cuBLAS reports its own failures through the call's status (lib.rs:387). */
 int wb_gemm_check(WbBackend* b);
 /* Test hook: one thread waits with the GEMM kernels' bounded barrier wait on a barrier nothing arrives at, gives up
  * after `polls` polls (1..2^20) and raises the same flag; the next wb_gemm_check then returns WB_ERR_TIMEOUT. */
 int wb_gemm_selftest_timeout(WbBackend* b, int polls);
+/* The same with the layer norm kernels' wait and flag. */
+int wb_layer_norm_selftest_timeout(WbBackend* b, int polls);
 
 /* A chain of unary / binary trait calls over one index space as ONE launch (no counterpart in the reference, which
  * launches each op by itself: crates/weta-cuda/src/lib.rs:482-521).  `inputs`: up to 8 f32 views of n elements each

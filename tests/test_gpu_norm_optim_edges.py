@@ -1,8 +1,11 @@
 """Layer norm, gradient norm and the many-tensor Adam at the edges of what their documentation allows, on the GPU."""
+import ctypes
+
 import numpy as np
 import pytest
 
 from weta_b200 import layers, optim
+from weta_b200.backend import B200Backend, BackendError
 from weta_b200.core import BinaryOp, DType, Layout
 from weta_b200.fusion import FusingBackend
 
@@ -113,3 +116,75 @@ def test_8_bit_step_with_subnormal_quotients_half_way_between_two(gpu, c):
     got = down(gpu, store, n)
     assert np.array_equal(got, -even.astype(F))
     assert same(got, Plain(n, 8).step(np.zeros(n, F), g, 1, lr, 0.0, 0.0, eps, 0.0, False, False, None))
+
+
+def norm_twice(be, n=512):
+    """A forward and a backward call that both wait for copies; the sum of their outputs' bits."""
+    rng = np.random.default_rng(n)
+    l, x = Layout.contiguous([7, n]), be.from_host(rng.standard_normal(7 * n).astype(F))
+    y, m, r = layers.layer_norm_fwd(be, x, l, DType.F32, 1)
+    dx, _, _ = layers.layer_norm_bwd(be, x, l, y, l, DType.F32, 1, None, m, r)
+    return down(be, y, 7 * n), down(be, dx, 7 * n)
+
+
+def test_a_wait_that_runs_out_is_seen_by_its_own_backend_only(gpu):
+    """The hook lets the kernels' bounded wait run out on one backend; another backend's check neither reports nor clears it,
+    and both go on working.  A GEMM's flag that is up at the same time is cleared by the same check."""
+    for f in (gpu.lib.wb_layer_norm_selftest_timeout, gpu.lib.wb_gemm_selftest_timeout):
+        f.argtypes, f.restype = [ctypes.c_void_p, ctypes.c_int], ctypes.c_int
+    be = B200Backend(0)
+    fresh = B200Backend(0)
+    before = norm_twice(be)
+    gpu.gemm_check()
+    be.gemm_check()
+    be.check(be.lib.wb_layer_norm_selftest_timeout(be.handle, 64))
+    be.synchronize()
+    norm_twice(gpu)
+    gpu.gemm_check()
+    fresh.gemm_check()
+    with pytest.raises(BackendError, match="layer norm gave up"):
+        be.gemm_check()
+    be.gemm_check()
+    be.check(be.lib.wb_layer_norm_selftest_timeout(be.handle, 64))
+    be.check(be.lib.wb_gemm_selftest_timeout(be.handle, 64))
+    with pytest.raises(BackendError, match="gave up") as e:
+        be.gemm_check()
+    assert e.value.status == 6
+    be.gemm_check()
+    for a, b in zip(before, norm_twice(be)):
+        assert np.array_equal(a, b)
+    be.gemm_check()
+    be.close()
+    fresh.close()
+
+
+def test_the_first_call_of_a_backend_may_be_captured(gpu):
+    """Whatever a backend needs for its waits is made without disturbing a capture."""
+    import torch
+
+    rows, n = 7, 9000
+    st = torch.cuda.Stream()
+    be = B200Backend(0, stream=st.cuda_stream)
+    t = {k: torch.zeros(s, device="cuda") for k, s in dict(x=(rows, n), y=(rows, n), m=(rows,), r=(rows,), dx=(rows, n)).items()}
+    torch.cuda.synchronize()
+    s = {k: be.wrap_pointer(a.data_ptr(), a.numel(), DType.F32) for k, a in t.items()}
+    l = Layout.contiguous([rows, n])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        layers.layer_norm_fwd(be, s["x"], l, DType.F32, 1, out=(s["y"], s["m"], s["r"]))
+        layers.layer_norm_bwd(be, s["x"], l, s["y"], l, DType.F32, 1, None, s["m"], s["r"], out=(s["dx"], None, None))
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((rows, n)).astype(F)
+    t["x"].copy_(torch.from_numpy(x))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        graph.replay()
+    torch.cuda.synchronize()
+    be.gemm_check()
+    xs = gpu.from_host(x.reshape(-1))
+    y, m, r = layers.layer_norm_fwd(gpu, xs, l, DType.F32, 1)
+    dx, _, _ = layers.layer_norm_bwd(gpu, xs, l, y, l, DType.F32, 1, None, m, r)
+    assert np.array_equal(t["y"].cpu().numpy().reshape(-1), down(gpu, y, rows * n))
+    assert np.array_equal(t["dx"].cpu().numpy().reshape(-1), down(gpu, dx, rows * n))
+    del graph
+    s.clear()

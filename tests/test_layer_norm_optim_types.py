@@ -85,3 +85,15 @@ def test_parameters_gradients_and_the_scale(other):
         optimizer().set_grads([storage(other, 10)])
     with pytest.raises(BackendError, match="scale is not a storage of f32"):
         optimizer().step(1, storage(other, 1))
+
+
+def test_the_wait_test_hook_refuses():
+    import ctypes
+
+    from weta_b200.backend import load_library
+
+    f = load_library().wb_layer_norm_selftest_timeout
+    f.argtypes, f.restype = [ctypes.c_void_p, ctypes.c_int], ctypes.c_int
+    handle = ctypes.create_string_buffer(1 << 16)
+    for args in ((None, 100), (handle, 0), (handle, -1), (handle, (1 << 20) + 1)):
+        assert f(*args) == 1

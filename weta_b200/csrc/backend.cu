@@ -74,6 +74,7 @@ extern "C" int wb_backend_destroy(WbBackend* b) {
     for (auto& kv : b->free_blocks) cudaFree(kv.second);
     if (b->scratch) cudaFree(b->scratch);
     if (b->narrow_counters) cudaFree(b->narrow_counters);
+    if (b->ln_gave_up) cudaFreeHost(b->ln_gave_up);
     if (b->own_stream) cudaStreamDestroy(b->stream);
     delete b;
     return WB_OK;

@@ -92,6 +92,8 @@ struct WbBackend {
     // 4096 block counters for kernels whose last block finishes a reduction (narrow_linear.cu, trainer.cu); every such
     // kernel finds them zero and leaves them zero
     void* narrow_counters = nullptr;
+    // raised by layer_norm.cu's kernels when a bounded wait runs out (pinned host memory, made on first use)
+    int* ln_gave_up = nullptr;
 };
 
 inline size_t wb_dtype_size(int dt) { return dt == WB_F32 ? 4 : 8; }

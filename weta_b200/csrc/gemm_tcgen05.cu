@@ -603,11 +603,11 @@ extern "C" int wb_gemm_selftest_timeout(WbBackend* b, int polls) {
     return WB_OK;
 }
 
-// Reads the device-side error flag the GEMM kernels raise when a bounded wait runs out.
+// Reads the error flags that the GEMM kernels and the layer norms raise when a bounded wait runs out, and clears both.
 // Synchronises the stream; meant for tests and for wb_synchronize-style checkpoints.
 extern "C" int wb_gemm_check(WbBackend* b) {
-    WB_TRY(wb_layer_norm_check(b));
-    if (!b->gemm_state) return WB_OK;
+    const int layer_norm = wb_layer_norm_check(b);
+    if (!b->gemm_state || (layer_norm != WB_OK && layer_norm != WB_ERR_TIMEOUT)) return layer_norm;
     GemmState* st = static_cast<GemmState*>(b->gemm_state);
     WB_CHECK_CUDA(cudaMemcpyAsync(st->error_host, st->error_flag, sizeof(int), cudaMemcpyDeviceToHost, b->stream));
     WB_CHECK_CUDA(cudaStreamSynchronize(b->stream));
@@ -616,7 +616,7 @@ extern "C" int wb_gemm_check(WbBackend* b) {
         wb_set_error("a tensor-core GEMM gave up waiting on a pipeline barrier");
         return WB_ERR_TIMEOUT;
     }
-    return WB_OK;
+    return layer_norm;
 }
 
 extern "C" int wb_matmul_into(WbBackend* b, const WbView* a, const WbView* bb, void* out) {

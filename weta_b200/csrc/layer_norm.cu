@@ -235,7 +235,6 @@ __global__ void __launch_bounds__(fwd_threads<TPR>) ln_fwd_rows_kernel(const T* 
 // outside the span is read.
 constexpr int MOST_RING = 4;
 constexpr uint32_t POLLS = 1u << 26;
-__device__ int g_ln_timeout;  // raised when a bounded wait runs out; read by wb_layer_norm_check
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void bar_init(uint64_t* bar) {
@@ -253,8 +252,8 @@ template <class T>
 __device__ __forceinline__ void copy_one(T* dst, const T* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(dst)), "l"(src), "n"(sizeof(T)) : "memory");
 }
-// Bounded: after `limit` polls the flag goes up, later waits give up sooner and the kernel runs to its end on what is there.
-__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, uint32_t& limit) {
+// Bounded: after `limit` polls the backend's flag (pinned host memory, read by wb_layer_norm_check) goes up, later waits give up sooner and the kernel runs to its end on what is there.
+__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, uint32_t& limit, int* gave_up) {
     const uint32_t addr = smem_addr(bar);
     for (uint32_t i = 0; i < limit; ++i) {
         uint32_t done;
@@ -265,7 +264,7 @@ __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, uint32_
         if (done) return;
     }
     limit = POLLS >> 10;
-    atomicExch(&g_ln_timeout, 1);
+    *reinterpret_cast<volatile int*>(gave_up) = 1;
 }
 
 template <class T>
@@ -327,6 +326,7 @@ struct SpanShape {
     int spans;
     int ring;  // slots
     int cap;   // elements of a slot's buffer
+    int* gave_up;
 };
 
 // A unit from shared memory: one 16-byte load, or (where the operand's rows start at another misalignment than the result's)
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
     uint32_t limit = POLLS, phase = 0;
     int slot = 0;
     for (int span = first; span < sh.spans; span += groups) {
-        bar_wait(&full[group][slot], phase, limit);
+        bar_wait(&full[group][slot], phase, limit, sh.gave_up);
         if (HALVES && span != first) fetch(span + (sh.ring - 1) * groups, slot == 0 ? sh.ring - 1 : slot - 1, 2);
         const int64_t row0 = static_cast<int64_t>(span) * sh.r;
         const int nr = static_cast<int>(min(static_cast<int64_t>(sh.r), sh.rows - row0));
@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
         const bool more = row < sh.spans;
         T s[2] = {0, 0};
         if (more) {
-            bar_wait(&full[slot], phase, limit);
+            bar_wait(&full[slot], phase, limit, sh.gave_up);
             const T mu = ring[slot * slot_elems + 2 * sh.cap - U], rs = ring[slot * slot_elems + 2 * sh.cap - U + 32];
             const Pair<T> minus_mu = pair(-mu, -mu), rs2 = pair(rs, rs);
             const bool far = far_from_zero(mu, rs);
@@ -960,7 +960,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_fwd_span_kernel(const T* _
     uint32_t limit = POLLS, phase = 0;
     int slot = 0;
     for (int row = first; row < sh.spans; row += groups) {
-        bar_wait(&full[slot], phase, limit);
+        bar_wait(&full[slot], phase, limit, sh.gave_up);
         const T* bx = ring + slot * sh.cap + col.u0 * U - col.mis - from + t * U;
         if (MODE != ALIGNED) bx += misalignment(x + static_cast<int64_t>(row) * sh.pitch_x + from);
         Pair<T> d[NV][H], s2 = pair(T(0), T(0));
@@ -1284,6 +1284,23 @@ cudaError_t allow_shared(int ordinal) {
     return e;
 }
 
+// The backend's flag, made by its first call that waits.  That call may be captured, and other threads may be capturing: the
+// allocation needs no stream, so this thread leaves their modes aside for it.
+int make_wait_flag(WbBackend* b) {
+    std::lock_guard<std::mutex> lock(b->mu);
+    if (!b->ln_gave_up) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        WB_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        void* p = nullptr;
+        const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable);
+        (void)cudaThreadExchangeStreamCaptureMode(&mode);
+        WB_CHECK_CUDA(e);
+        *static_cast<int*>(p) = 0;
+        b->ln_gave_up = static_cast<int*>(p);
+    }
+    return WB_OK;
+}
+
 // The grid of a span kernel: as many groups as the device holds at a time or as there are spans, and a multiple of the
 // period, so that a group's rows are all of one misalignment.  Where one block with at most `few` spans per group will do, or
 // up to `joint` of them, they leave the sums themselves, the latter as a cluster, and *slabs is 1: that saves the launch that
@@ -1384,6 +1401,7 @@ bool bwd_spans(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t p
     const int64_t units = (s.cols + UNIT<T> - 1 + (aligned ? 0 : UNIT<T> - 1)) / UNIT<T>;
     const bool cut = !aligned || s.cols % UNIT<T> != 0;
     SpanShape sh;
+    sh.gave_up = b->ln_gave_up;
     sh.rows = s.rows;
     sh.cols = static_cast<int>(s.cols);
     sh.pitch_x = pitch_x;
@@ -1464,6 +1482,7 @@ bool fwd_spans(WbBackend* b, const T* x, int64_t pitch, const Shape& s, const T*
     auto go = [&](auto nv, auto cl, auto mode) {
         constexpr int NV = decltype(nv)::value, CL = decltype(cl)::value;
         SpanShape sh{};
+        sh.gave_up = b->ln_gave_up;
         sh.rows = s.rows;
         sh.cols = static_cast<int>(s.cols);
         sh.pitch_x = pitch;
@@ -1581,19 +1600,33 @@ int64_t bwd_workspace(int sm_count, int64_t rows, int64_t cols, int dtype) {
 
 }  // namespace
 
-// Reads and clears the flag of the bounded waits above; waits for the stream.
+// Reads and clears the flag of the backend's bounded waits; waits for the stream.  The exchange loses none that goes up meanwhile.
 int wb_layer_norm_check(WbBackend* b) {
-    WbDeviceGuard dev(b->ordinal);
-    WB_CHECK_CUDA(dev.status);
-    int raised = 0;
-    WB_CHECK_CUDA(cudaMemcpyFromSymbolAsync(&raised, g_ln_timeout, sizeof(int), 0, cudaMemcpyDeviceToHost, b->stream));
+    if (!b->ln_gave_up) return WB_OK;  // no call of this backend has waited
     WB_CHECK_CUDA(cudaStreamSynchronize(b->stream));
-    if (!raised) return WB_OK;
-    const int zero = 0;
-    WB_CHECK_CUDA(cudaMemcpyToSymbolAsync(g_ln_timeout, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, b->stream));
-    WB_CHECK_CUDA(cudaStreamSynchronize(b->stream));
+    if (__atomic_exchange_n(b->ln_gave_up, 0, __ATOMIC_ACQ_REL) == 0) return WB_OK;
     wb_set_error("a layer norm gave up waiting for a bulk copy");
     return WB_ERR_TIMEOUT;
+}
+
+// One thread waits, the way the kernels above do, on a barrier that nothing arrives at (no copy is in flight), and gives up.
+__global__ void ln_timeout_selftest_kernel(int* gave_up, uint32_t polls) {
+    __shared__ uint64_t bar;
+    if (threadIdx.x == 0) {
+        bar_init(&bar);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        bar_wait(&bar, 0, polls, gave_up);
+    }
+}
+
+extern "C" int wb_layer_norm_selftest_timeout(WbBackend* b, int polls) {
+    WB_REQUIRE(b && polls > 0 && polls <= (1 << 20), WB_ERR_INVALID, "wb_layer_norm_selftest_timeout: polls must be 1..2^20");
+    WbDeviceGuard dev(b->ordinal);
+    WB_CHECK_CUDA(dev.status);
+    WB_TRY(make_wait_flag(b));
+    ln_timeout_selftest_kernel<<<1, 32, 0, b->stream>>>(b->ln_gave_up, static_cast<uint32_t>(polls));
+    WB_LAUNCH_OK(b);
+    return WB_OK;
 }
 
 // ---- entry points ------------------------------------------------------------------------------------------
@@ -1616,6 +1649,7 @@ extern "C" int wb_layer_norm_fwd(WbBackend* b, const WbView* x, int normalized_d
     WB_REQUIRE(!wb_spans_clash(spans.s, spans.n), WB_ERR_INVALID, "wb_layer_norm_fwd: an output overlaps another operand");
     WbDeviceGuard dev(b->ordinal);
     WB_CHECK_CUDA(dev.status);
+    WB_TRY(make_wait_flag(b));
     WbProfileScope ps(b, "layer_norm");
     if (x->dtype == WB_F32)
         return fwd_typed<float>(b, x, normalized_dims, s, static_cast<const float*>(weight), static_cast<const float*>(bias), eps,
@@ -1665,6 +1699,7 @@ extern "C" int wb_layer_norm_bwd(WbBackend* b, const WbView* x, const WbView* dy
                "wb_layer_norm_bwd: an output overlaps another operand");
     WbDeviceGuard dev(b->ordinal);
     WB_CHECK_CUDA(dev.status);
+    WB_TRY(make_wait_flag(b));
     WbProfileScope ps(b, "layer_norm_bwd");
     if (s.rows == 0) {  // the sums over no rows
         if (dweight) WB_CHECK_CUDA(cudaMemsetAsync(dweight, 0, static_cast<size_t>(s.cols * size), b->stream));
