@@ -188,3 +188,53 @@ def test_the_first_call_of_a_backend_may_be_captured(gpu):
     assert np.array_equal(t["dx"].cpu().numpy().reshape(-1), down(gpu, dx, rows * n))
     del graph
     s.clear()
+
+
+ROWS = [(1, 1), (1, 1024), (2, 64), (3, 7), (5, 9001), (7, 96), (33, 1000), (128, 512), (297, 40), (1000, 33), (2500, 256), (4099, 100), (70001, 3), (3001, 777),
+        (1201, 2048), (1111, 4100), (1400, 4096), (700, 8192), (601, 9000), (400, 9001), (330, 16388), (20011, 33), (9000, 250), (6007, 130),
+        (4443, 1000), (2368, 12), (300, 20001), (90, 33000)]
+
+
+@pytest.mark.parametrize("dt", [DType.F32, DType.F64])
+@pytest.mark.parametrize("rows,cols", ROWS)
+@pytest.mark.parametrize("form", ["plain", "shifted", "strided"])
+def test_each_row_counts_once_in_the_sums(gpu, rows, cols, dt, form):
+    """Small whole numbers, mean 1 or 2, rstd 1: every partial sum of dweight and dbias is a whole number under 2^24 and exact in
+    any order, and every row adds at least 1 to every column, so a row left out or taken twice shows in each."""
+    if form == "strided" and rows * cols > 1 << 20:
+        pytest.skip("the kernel for any view is covered by the smaller shapes")
+    rng = np.random.default_rng(rows + cols)
+    t = NP[dt]
+    mean = rng.integers(1, 3, rows)
+    x = mean[:, None] + rng.integers(1, 4, (rows, cols))
+    dy = rng.integers(1, 3, (rows, cols))
+    assert 6 * rows < 1 << 24
+    dw, db = (dy * (x - mean[:, None])).sum(0), dy.sum(0)
+    lx = lg = Layout.contiguous([rows, cols])
+    xs, gs = x.astype(t).reshape(-1), dy.astype(t).reshape(-1)
+    if form == "shifted":
+        gs, lg = np.concatenate([np.zeros(1, t), gs]), Layout([rows, cols], [cols, 1], 1)
+    if form == "strided":
+        xs, lx = np.ascontiguousarray(x.astype(t).T).reshape(-1), Layout([rows, cols], [1, rows], 0)
+    args = (gpu, gpu.from_host(xs), lx, gpu.from_host(gs), lg, dt, 1, None, gpu.from_host(mean.astype(t)), gpu.from_host(np.ones(rows, t)))
+    for out in (None, (None, gpu.alloc(cols, dt), gpu.alloc(cols, dt))):
+        _, w, b = layers.layer_norm_bwd(*args, out=out)
+        assert np.array_equal(down(gpu, w, cols, dt), dw.astype(t)) and np.array_equal(down(gpu, b, cols, dt), db.astype(t))
+
+
+@pytest.mark.parametrize("rows,cols", [s for s in ROWS if s[1] <= 8192])
+def test_sums_over_rows_are_added_in_short_chains(gpu, rows, cols):
+    """Rows of up to 8192 f32 columns.  A thread adds the terms of at most rows / 148 rows beyond one span of its block (32 rows),
+    or of three spans where few blocks run; the block joins at most 64 threads per column in f32, the blocks at most eight in f32
+    (a cluster) or all of them in f64, and a term is rounded three times itself: (rows / 148 + 96 + 64 + 8 + 4) u of the sum of
+    magnitudes."""
+    rng = np.random.default_rng(rows * 3 + cols)
+    x, dy = (rng.standard_normal((rows, cols)).astype(F) for _ in range(2))
+    mean, rstd = (rng.standard_normal(rows) * 0.1).astype(F), rng.uniform(0.5, 2, rows).astype(F)
+    l = Layout.contiguous([rows, cols])
+    _, dw, db = layers.layer_norm_bwd(gpu, gpu.from_host(x.reshape(-1)), l, gpu.from_host(dy.reshape(-1)), l, DType.F32, 1, None, gpu.from_host(mean),
+                                      gpu.from_host(rstd))
+    terms = dy.astype(np.float64) * ((x.astype(np.float64) - mean[:, None]) * rstd[:, None])
+    chain = (rows / 148 + 172) * 2.0 ** -24
+    assert (np.abs(down(gpu, dw, cols) - terms.sum(0)) <= chain * np.abs(terms).sum(0)).all()
+    assert (np.abs(down(gpu, db, cols) - dy.sum(0, dtype=np.float64)) <= chain * np.abs(dy).sum(0, dtype=np.float64)).all()
