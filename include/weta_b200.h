@@ -420,6 +420,11 @@ int wb_adam_multi_grad_norm(WbAdamMulti* h, double max_norm, float* norm, float*
 int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64_t t, double grad_scale, const float* device_grad_scale);
 /* The moments as f32 [P] each (either may be NULL), in the state's order: what 8-bit state stands for. */
 int wb_adam_multi_read_state(WbAdamMulti* h, float* m, float* v);
+/* Test hook: how many values of the range that the 8-bit step's own root, reciprocal and quotient are used in differ from the
+ * correctly rounded result: wrong[0] roots (every f32 in [2^-100, 2^80]), wrong[1] reciprocals (every f32 in [2^-60, 2^61]),
+ * wrong[2] quotients (four numerators for every denominator); wrong[3]: the roots and reciprocals looked at.  Waits for the
+ * stream. */
+int wb_adam_multi_selftest_rounding(WbBackend* b, int64_t* wrong);
 
 /* ---- data-parallel training step ---------------------------------------------------------------
  * No counterpart in the reference: its backends are per-ordinal singletons with no gradient exchange

@@ -238,3 +238,13 @@ def test_sums_over_rows_are_added_in_short_chains(gpu, rows, cols):
     chain = (rows / 148 + 172) * 2.0 ** -24
     assert (np.abs(down(gpu, dw, cols) - terms.sum(0)) <= chain * np.abs(terms).sum(0)).all()
     assert (np.abs(down(gpu, db, cols) - dy.sum(0, dtype=np.float64)) <= chain * np.abs(dy).sum(0, dtype=np.float64)).all()
+
+
+def test_roots_reciprocals_and_quotients_of_the_8_bit_step_are_rounded(gpu):
+    """Every root and reciprocal of the range that the step uses them in, and four billion quotients."""
+    f = gpu.lib.wb_adam_multi_selftest_rounding
+    f.argtypes, f.restype = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64)], ctypes.c_int
+    wrong = (ctypes.c_int64 * 4)(-1, -1, -1, -1)
+    gpu.check(f(gpu.handle, wrong))
+    assert list(wrong) == [0, 0, 0, (180 + 121) * 2 ** 23 + 4]  # two at a time, both ends included
+    assert f(None, wrong) == 1 and f(gpu.handle, None) == 1

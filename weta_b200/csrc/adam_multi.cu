@@ -153,7 +153,11 @@ __device__ __forceinline__ float decode_root(float c, float unit) { return c * c
 // caller sends all others to sqrtf and /): an approximation from the function unit, refined, then corrected by its exact
 // residual with one fused operation (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
 // processor", IBM J. Res. Dev. 34, 1990: with 1/d correctly rounded and q within a unit, q + (m - d q) / d rounds to m/d).
-// That the reciprocal is correctly rounded, and the root, was checked for every mantissa (and both parities of the exponent).
+// That the root and the reciprocal are correctly rounded is checked for every value of the range they are used in
+// (wb_adam_multi_selftest_rounding, which a test calls).
+constexpr float LOW_M = 8.6736173798840355e-19f, TOP_M = 1.152921504606847e18f;   // 2^-60 and 2^60
+constexpr float LOW_V = 7.8886090522101181e-31f, TOP_V = 1.2089258196146292e24f;  // 2^-100 and 2^80
+constexpr float LOW_D = LOW_M, TOP_D = 2.305843009213694e18f;                     // 2^-60 and 2^61
 __device__ __forceinline__ Pair<float> root_of(const Pair<float>& v) {
     float a, b, ya, yb;
     unpair(v, a, b);
@@ -162,15 +166,18 @@ __device__ __forceinline__ Pair<float> root_of(const Pair<float>& v) {
     const Pair<float> y = pair(ya, yb), g = v * y, minus_v = v * pair(-1.f, -1.f), minus_half = y * pair(-0.5f, -0.5f);
     return muladd(muladd(g, g, minus_v), minus_half, g);
 }
-// m / d from -d.
-__device__ __forceinline__ Pair<float> quotient_of(const Pair<float>& m, const Pair<float>& minus_d) {
+// 1 / d from -d.
+__device__ __forceinline__ Pair<float> reciprocal_of(const Pair<float>& minus_d) {
     float a, b, ya, yb;
     unpair(minus_d, a, b);
     asm("rcp.approx.f32 %0, %1;" : "=f"(ya) : "f"(-a));
     asm("rcp.approx.f32 %0, %1;" : "=f"(yb) : "f"(-b));
-    Pair<float> y = pair(ya, yb);
-    y = muladd(muladd(minus_d, y, pair(1.f, 1.f)), y, y);
-    const Pair<float> q = m * y;
+    const Pair<float> y = pair(ya, yb);
+    return muladd(muladd(minus_d, y, pair(1.f, 1.f)), y, y);
+}
+// m / d from -d.
+__device__ __forceinline__ Pair<float> quotient_of(const Pair<float>& m, const Pair<float>& minus_d) {
+    const Pair<float> y = reciprocal_of(minus_d), q = m * y;
     return muladd(muladd(minus_d, q, m), y, q);
 }
 
@@ -340,8 +347,7 @@ __global__ void __launch_bounds__(THREADS, 5) adam_multi8_kernel(const __grid_co
     }
     // m in [2^-60, 2^60], v in [2^-100, 2^80], eps in [2^-60, 2^60] and 1 / sqrt(1 - beta2^t) at most 2^20: the denominator lies in
     // [2^-60, 2^61] and the quotient in [2^-121, 2^120], so nothing leaves the normal range before the quotient is multiplied
-    if (k8.eps_normal && low_m >= 8.6736173798840355e-19f && low_v >= 7.8886090522101181e-31f && top_m <= 1.152921504606847e18f &&
-        top_v <= 1.2089258196146292e24f) {
+    if (k8.eps_normal && low_m >= LOW_M && low_v >= LOW_V && top_m <= TOP_M && top_v <= TOP_V) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             root[j] = root_of(root[j]);
@@ -426,6 +432,40 @@ __global__ void __launch_bounds__(THREADS) adam_multi8_read_kernel(const uint32_
         }
         put(v, a);
     }
+}
+
+// Counts the values of the fast path's range whose root or reciprocal is not the rounded one, quotients of four numerators
+// for each denominator, and last all roots and reciprocals that were looked at.
+__global__ void __launch_bounds__(THREADS) adam_rounding_selftest_kernel(unsigned long long* bad) {
+    const uint32_t stride = gridDim.x * THREADS, first = blockIdx.x * THREADS + threadIdx.x;
+    unsigned long long roots = 0, reciprocals = 0, quotients = 0, seen = 0;
+    auto differ = [](const Pair<float>& p, float x, float y) {
+        float a, b;
+        unpair(p, a, b);
+        return (__float_as_uint(a) != __float_as_uint(x)) + (__float_as_uint(b) != __float_as_uint(y));
+    };
+    for (uint32_t i = __float_as_uint(LOW_V) + 2 * first; i <= __float_as_uint(TOP_V); i += 2 * stride) {
+        const float a = __uint_as_float(i), b = __uint_as_float(i + 1);
+        roots += differ(root_of(pair(a, b)), sqrtf(a), sqrtf(b));
+        seen += 2;
+    }
+    for (uint32_t i = __float_as_uint(LOW_D) + 2 * first; i <= __float_as_uint(TOP_D); i += 2 * stride) {
+        const float a = __uint_as_float(i), b = __uint_as_float(i + 1);
+        const Pair<float> minus_d = pair(-a, -b);
+        reciprocals += differ(reciprocal_of(minus_d), 1.f / a, 1.f / b);
+        seen += 2;
+        uint32_t h = i * 2654435761u;
+        for (int k = 0; k < 4; ++k) {  // numerators of any mantissa and sign, exponents -60 to 59
+            h = h * 1664525u + 1013904223u;
+            const uint32_t e = (67u + (h >> 8) % 120u) << 23;
+            const float m = __uint_as_float((h & 0x807fffffu) | e), n = __uint_as_float(((h * 40503u) & 0x807fffffu) | e);
+            quotients += differ(quotient_of(pair(m, n), minus_d), m / a, n / b);
+        }
+    }
+    atomicAdd(bad, roots);
+    atomicAdd(bad + 1, reciprocals);
+    atomicAdd(bad + 2, quotients);
+    atomicAdd(bad + 3, seen);
 }
 
 // ---- the norm -----------------------------------------------------------------------------------------------
@@ -762,7 +802,7 @@ extern "C" int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64
     k8.inv_sqrt_bc2 = k.inv_sqrt_bc2;
     k8.eps = k.eps;
     k8.step = k.step_size;
-    k8.eps_normal = k.eps >= 8.6736173798840355e-19f && k.eps <= 1.152921504606847e18f && k.inv_sqrt_bc2 <= 1048576.f;
+    k8.eps_normal = k.eps >= LOW_M && k.eps <= TOP_M && k.inv_sqrt_bc2 <= 1048576.f;
     k8.minus_step = twice(-k.step_size);
     k8.minus_zero = twice(-0.f);
     k8.gscale = k.scale_grad ? k.gscale : 1.f;
@@ -814,5 +854,27 @@ extern "C" int wb_adam_multi_read_state(WbAdamMulti* h, float* m, float* v) {
                                 reinterpret_cast<const uint32_t*>(state), reinterpret_cast<const uint32_t*>(state + p), scales, scales + p / BLOCK8, m, v,
                                 groups, wide));
     WB_LAUNCH_OK(b);
+    return WB_OK;
+}
+
+extern "C" int wb_adam_multi_selftest_rounding(WbBackend* b, int64_t* wrong) {
+    WB_REQUIRE(b && wrong, WB_ERR_INVALID, "wb_adam_multi_selftest_rounding: null pointer");
+    WbDeviceGuard dev(b->ordinal);
+    WB_CHECK_CUDA(dev.status);
+    void* counts = nullptr;
+    size_t klass = 0;
+    WB_TRY(wb_arena_alloc(b, 4 * sizeof(int64_t), &counts, &klass));
+    cudaError_t e = cudaMemsetAsync(counts, 0, 4 * sizeof(int64_t), b->stream);
+    if (e == cudaSuccess) {
+        adam_rounding_selftest_kernel<<<8 * b->sm_count, THREADS, 0, b->stream>>>(static_cast<unsigned long long*>(counts));
+        b->launches++;
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess) {
+        e = cudaMemcpyAsync(wrong, counts, 4 * sizeof(int64_t), cudaMemcpyDeviceToHost, b->stream);
+    }
+    if (e == cudaSuccess) e = cudaStreamSynchronize(b->stream);
+    wb_arena_free(b, counts, klass);
+    WB_CHECK_CUDA(e);
     return WB_OK;
 }
