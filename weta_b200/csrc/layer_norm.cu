@@ -1209,26 +1209,29 @@ bool rows_aligned(const void* p, int64_t pitch, int64_t cols) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch % wide<T> == 0 && cols % wide<T> == 0;
 }
 
-// Calls f with (threads per row, vectors per thread) for rows of `packs` vectors, at most MOST vectors per thread: the
-// fewest threads that hold the row, so that small rows share a block and the reductions stay short.
-template <int MOST, int LEAST, class F>
+// Calls f with (threads per row, vectors per thread) for rows of `packs` vectors, at most MOST vectors per thread and at most
+// THREADS_MOST threads: the fewest threads that hold the row, so that small rows share a block and the reductions stay short.
+template <int MOST, int LEAST, int THREADS_MOST, class F>
 bool choose_row(int64_t packs, F&& f) {
     auto per = [&](auto tpr) -> bool {
         constexpr int TPR = decltype(tpr)::value;
-        if (packs > static_cast<int64_t>(TPR) * MOST) return false;
-        const int64_t nv = (packs + TPR - 1) / TPR;
-        if constexpr (TPR < LEAST) return false;
-        if constexpr (TPR == LEAST) {
-            if (nv <= 1) return f(tpr, std::integral_constant<int, 1>{}), true;
-            if (nv <= 2) return f(tpr, std::integral_constant<int, 2>{}), true;
-            if constexpr (MOST / 4 > 2)
-                if (nv <= MOST / 4) return f(tpr, std::integral_constant<int, MOST / 4>{}), true;
-            if constexpr (MOST / 2 > 2)
-                if (nv <= MOST / 2) return f(tpr, std::integral_constant<int, MOST / 2>{}), true;
+        if constexpr (TPR < LEAST || TPR > THREADS_MOST) {
+            return false;
+        } else {
+            if (packs > static_cast<int64_t>(TPR) * MOST) return false;
+            const int64_t nv = (packs + TPR - 1) / TPR;
+            if constexpr (TPR == LEAST) {
+                if (nv <= 1) return f(tpr, std::integral_constant<int, 1>{}), true;
+                if (nv <= 2) return f(tpr, std::integral_constant<int, 2>{}), true;
+                if constexpr (MOST / 4 > 2)
+                    if (nv <= MOST / 4) return f(tpr, std::integral_constant<int, MOST / 4>{}), true;
+                if constexpr (MOST / 2 > 2)
+                    if (nv <= MOST / 2) return f(tpr, std::integral_constant<int, MOST / 2>{}), true;
+            }
+            if constexpr (MOST >= 4)
+                if (nv <= MOST * 3 / 4) return f(tpr, std::integral_constant<int, MOST * 3 / 4>{}), true;
+            return f(tpr, std::integral_constant<int, MOST>{}), true;
         }
-        if constexpr (MOST >= 4)
-            if (nv <= MOST * 3 / 4) return f(tpr, std::integral_constant<int, MOST * 3 / 4>{}), true;
-        return f(tpr, std::integral_constant<int, MOST>{}), true;
     };
     return per(std::integral_constant<int, 8>{}) || per(std::integral_constant<int, 16>{}) || per(std::integral_constant<int, 32>{}) ||
            per(std::integral_constant<int, 64>{}) || per(std::integral_constant<int, 128>{}) || per(std::integral_constant<int, 256>{}) ||
@@ -1238,10 +1241,10 @@ bool choose_row(int64_t packs, F&& f) {
 template <class T>
 constexpr int row_elems = 64 / static_cast<int>(sizeof(T));  // elements of a row that a thread holds at most
 
-// MOST elements per thread.
+// MOST elements per thread.  Aligned rows that 512 threads do not hold go to fwd_spans.
 template <class T, int VEC, int MOST>
 bool fwd_rows(WbBackend* b, const T* x, int64_t pitch, const Shape& s, const T* w, const T* bias, double eps, T* y, T* mean, T* rstd, cudaError_t* err) {
-    return choose_row<MOST / VEC, 8>((s.cols + VEC - 1) / VEC, [&](auto tpr, auto nv) {
+    return choose_row<MOST / VEC, 8, VEC == 1 ? 1024 : 512>((s.cols + VEC - 1) / VEC, [&](auto tpr, auto nv) {
         constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, G = fwd_threads<TPR> / TPR;
         const int64_t grid = (s.rows + G - 1) / G;
         *err = wb_launch_pdl(ln_fwd_rows_kernel<T, VEC, TPR, NV>, dim3(static_cast<unsigned>(grid)), dim3(fwd_threads<TPR>), 0, b->stream, x, pitch,
@@ -1434,7 +1437,8 @@ bool bwd_spans(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t p
                                                                 ref, dx, parts, dw, db);
         return true;
     };
-    if ((cut || !same) && s.cols <= 16 * 4 * UNIT<T>) {
+    constexpr int SHORT = 16 * 4 * UNIT<T>;
+    if ((cut || !same) && s.cols <= SHORT) {
         const int nv = static_cast<int>((s.cols + (s.cols <= 8 * 4 * UNIT<T> ? 8 : 16) * UNIT<T> - 1) / ((s.cols <= 8 * 4 * UNIT<T> ? 8 : 16) * UNIT<T>));
         using M = std::integral_constant<int, ELEMENTS>;
         using N1 = std::integral_constant<int, 1>;
@@ -1450,7 +1454,8 @@ bool bwd_spans(WbBackend* b, const T* x, int64_t pitch_x, const T* dy, int64_t p
         return true;
     }
     const bool done = choose_span(units, dense && !cut && same, [&](auto tpr, auto nv) {
-        if constexpr (decltype(tpr)::value >= 32) {
+        static_assert(SHORT >= 32 * 2 * UNIT<T>, "rows that two units of a warp hold go by elements where they are cut");
+        if constexpr (decltype(tpr)::value > 32 || (decltype(tpr)::value == 32 && decltype(nv)::value > 2)) {
             if (!same) return go(tpr, nv, std::integral_constant<int, MIXED>{});
             if (cut) return go(tpr, nv, std::integral_constant<int, SHIFTED>{});
         }
