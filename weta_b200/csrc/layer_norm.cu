@@ -252,7 +252,8 @@ template <class T>
 __device__ __forceinline__ void copy_one(T* dst, const T* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(dst)), "l"(src), "n"(sizeof(T)) : "memory");
 }
-// Bounded: after `limit` polls the backend's flag (pinned host memory, read by wb_layer_norm_check) goes up, later waits give up sooner and the kernel runs to its end on what is there.
+// Bounded: after `limit` polls the backend's flag (pinned host memory, read by wb_layer_norm_check) goes up, later waits give up
+// sooner and the kernel runs to its end on what is there.
 __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, uint32_t& limit, int* gave_up) {
     const uint32_t addr = smem_addr(bar);
     for (uint32_t i = 0; i < limit; ++i) {
@@ -299,6 +300,44 @@ __device__ __forceinline__ void fetch_ends(T* buf, const T* p, int n, int k) {
     const Split<T> s(p, n);
     const int i = k < 4 ? k : s.head + s.mid + k - 4;
     if (k < 4 ? k < s.head : k - 4 < s.tail) copy_one(buf + s.mis + i, p + i);
+}
+
+// How rows lie to 16-byte boundaries.  ALIGNED: every row of x, dy and the result starts and ends on one, so no unit is cut.
+// The others cut units at the rows' ends.  SHIFTED: the three share each row's misalignment and a slot holds one row; the other
+// places of its first and last unit hold the row's mean (x) and zeros (dy), so that xhat and the gradient are 0 there.  MIXED:
+// they do not share it; x and dy are read from shared memory element by element, and a cut unit's foreign elements are
+// replaced.  ELEMENTS, for rows so short that a span of one row would be all overhead: no units, thread t holds the columns t,
+// t + TPR, ... of rows of any misalignment.
+enum { ALIGNED, SHIFTED, MIXED, ELEMENTS };
+
+// The small copies of a row of n columns by the lanes of a warp, one each: the ends of x (lanes 0 to 7) and of dy (8 to 15), the
+// row's mean into the other places of x's first and last unit (SHIFTED, 16 to 23), its rstd to stats + 32 (24) and its mean to
+// the first unit of `stats` (25 on).  Where the misalignment stays the same, so does all of this but the row.
+template <class T>
+struct SmallCopy {
+    bool on = false;
+    int to = 0;  // in the slot
+    const T* from = nullptr;
+};
+template <class T, int MODE>
+__device__ __forceinline__ SmallCopy<T> small_copy(const T* x, const T* dy, int n, int at_dy, int stats, const T* mean, const T* rstd, int lane) {
+    SmallCopy<T> c;
+    if constexpr (MODE != ALIGNED) {
+        const bool of_g = lane >= 8 && lane < 16, gap = lane >= 16, tail = lane & 4;
+        const T* p = of_g ? dy : x;
+        const Split<T> s(p, n);
+        const int end = s.mis + n, i = lane & 3;
+        const int place = i + (gap ? (tail ? end : 0) : s.mis + (tail ? s.head + s.mid : 0));
+        c.on = i < (gap ? (MODE == SHIFTED ? (tail ? -end & (UNIT<T> - 1) : s.mis) : 0) : tail ? s.tail : s.head);
+        c.to = (of_g ? at_dy : 0) + place;
+        c.from = gap ? mean : p + place - s.mis;
+    }
+    if (lane >= 24) {
+        c.on = lane < 25 + UNIT<T>;
+        c.to = stats + (lane == 24 ? 32 : lane - 25);
+        c.from = lane == 24 ? rstd : mean;
+    }
+    return c;
 }
 
 // Which columns a thread holds.  A row is cut into the 16-byte units of the result's memory: unit u of a row that starts `mis`
@@ -377,11 +416,6 @@ __device__ __forceinline__ void replace_outside(int c, int cols, const T& with, 
     }
 }
 
-// Whether (0 - mean) rstd is not finite.  Places that are not of a row hold zeros in the backward pass (MIXED: the row's mean);
-// their weight is zero, but zero times an infinity is not: in such a row (equal values of 2e36, say) they are left out.
-__device__ __forceinline__ bool far_from_zero(float mean, float rstd) { return !(fabsf(mean * rstd) <= 3.402823466e38f); }
-__device__ __forceinline__ bool far_from_zero(double mean, double rstd) { return !(fabs(mean * rstd) <= 1.7976931348623157e308); }
-
 constexpr int SPAN_THREADS = 512;
 constexpr int MOST_SHARED = 216 << 10;
 
@@ -431,12 +465,6 @@ __device__ __forceinline__ void cluster_sum(T (&s)[K], T (*peers)[CL][2], int ra
 // Backward.  TPR threads hold a row; narrower rows share a warp.  The weight's and the bias's gradients of a thread's columns
 // stay in its registers over all rows it sees; at the end the threads of a column are joined in shared memory and the block
 // leaves one row of partials.
-// How rows lie to 16-byte boundaries.  ALIGNED: every row of x, dy and the result starts and ends on one, so no unit is cut.
-// The others cut units at the rows' ends.  SHIFTED: the three share each row's misalignment and a slot holds one row, between
-// zeros that no copy writes over.  MIXED: they do not share it; x and dy are read from shared memory element by element, and a
-// cut unit's foreign elements are replaced.  ELEMENTS, for rows so short that a span of one row would be all overhead: no
-// units, thread t holds the columns t, t + TPR, ... of rows of any misalignment.
-enum { ALIGNED, SHIFTED, MIXED, ELEMENTS };
 template <class T, int TPR, int NV, int MODE>
 __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* __restrict__ x, const T* __restrict__ dy, const SpanShape sh,
                                                                      const T* __restrict__ w, const T* __restrict__ mean,
@@ -468,9 +496,9 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
     if (threadIdx.x < U) zeros[threadIdx.x] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncthreads();
-    if constexpr (MODE == SHIFTED) {  // the ends of each buffer: a unit before and after the first, all from the last on
-        for (int k = 0; k < 2 * sh.ring && g < 32; ++k) {
-            T* buf = ring + k / 2 * slot_elems + k % 2 * sh.cap;
+    if constexpr (MODE == SHIFTED) {  // the ends of each buffer of dy: a unit before and after the first, all from the last on
+        for (int k = 0; k < sh.ring && g < 32; ++k) {
+            T* buf = ring + k * slot_elems + sh.cap;
             const int e = g < 2 * U ? g - U : max(U, sh.cols - U) + g - 2 * U;
             if (e < sh.cap - U) buf[e] = 0;
         }
@@ -508,10 +536,15 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
                 if (part != 1) fetch_units(base + sh.cap, pg, sg, &full[group][slot]);
             }
             if (part != 2) {
-                if (MODE != ALIGNED && g < 16) fetch_ends(base + (g < 8 ? 0 : sh.cap), g < 8 ? px : pg, n, g & 7);
-                if (g < nr) {
-                    copy_one(base + 2 * sh.cap - U + g, mean + row0 + g);
-                    copy_one(base + 2 * sh.cap - U + 32 + g, rstd + row0 + g);
+                if constexpr (MODE == SHIFTED || MODE == MIXED) {  // spans of one row
+                    const SmallCopy<T> c = small_copy<T, MODE>(px, pg, n, sh.cap, 2 * sh.cap - U, mean + row0, rstd + row0, g);
+                    if (c.on) copy_one(base + c.to, c.from);
+                } else {
+                    if (MODE == ELEMENTS && g < 16) fetch_ends(base + (g < 8 ? 0 : sh.cap), g < 8 ? px : pg, n, g & 7);
+                    if (g < nr) {
+                        copy_one(base + 2 * sh.cap - U + g, mean + row0 + g);
+                        copy_one(base + 2 * sh.cap - U + 32 + g, rstd + row0 + g);
+                    }
                 }
             }
         }
@@ -552,6 +585,8 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
             const T *bx = span_x + r * sh.cols, *bg = span_g + r * sh.cols;
             const T mu = base[2 * sh.cap - U + r], rs = base[2 * sh.cap - U + 32 + r];
             const Pair<T> minus_mu = pair(-mu, -mu), rs2 = pair(rs, rs);
+            // xhat is 0 where there is no column: (0 - mu) rs may be infinite, which no weight makes nothing of
+            const Pair<T> minus_last = MODE == MIXED || MODE == ELEMENTS || col.some(NV - 1) ? minus_mu : pair(T(0), T(0));
             Pair<T> xh[NV][H], gv[NV][H], s0 = pair(T(0), T(0)), s1 = s0;
             auto take = [&](auto edges) {
 #pragma unroll
@@ -562,7 +597,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
                         for (int i = 0; i < H; ++i) {
                             const int c = column(j, 2 * i), d = column(j, 2 * i + 1);
                             const bool a = c < sh.cols, b = d < sh.cols;
-                            xh[j][i] = pair(a ? bx[c] : T(0), b ? bx[d] : T(0));
+                            xh[j][i] = pair(a ? bx[c] : mu, b ? bx[d] : mu);
                             up[i] = pair(a ? bg[c] : T(0), b ? bg[d] : T(0));
                         }
                     } else {
@@ -578,7 +613,7 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
                     }
 #pragma unroll
                     for (int i = 0; i < H; ++i) {
-                        xh[j][i] = (xh[j][i] + minus_mu) * rs2;
+                        xh[j][i] = (xh[j][i] + (j < NV - 1 ? minus_mu : minus_last)) * rs2;
                         gv[j][i] = up[i] * wv[j][i];
                         aw[j][i] = muladd(up[i], xh[j][i], aw[j][i]);
                         ab[j][i] = ab[j][i] + up[i];
@@ -593,18 +628,6 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_span_kernel(const T* _
             }
             if (!dx) continue;
             T s[2], lo, hi;
-            if (MODE != MIXED && far_from_zero(mu, rs)) {
-                s1 = pair(T(0), T(0));
-#pragma unroll
-                for (int j = 0; j < NV; ++j)
-#pragma unroll
-                    for (int i = 0; i < H; ++i) {
-                        const int c = column(j, 2 * i), d = column(j, 2 * i + 1);
-                        unpair(xh[j][i], lo, hi);
-                        const Pair<T> x2 = pair(c >= 0 && c < sh.cols ? lo : T(0), d >= 0 && d < sh.cols ? hi : T(0));
-                        if (live) s1 = muladd(gv[j][i], x2, s1);
-                    }
-            }
             unpair(s0, lo, hi);
             s[0] = lo + hi;
             unpair(s1, lo, hi);
@@ -732,8 +755,8 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
     __syncthreads();
     cluster_sync();
     if constexpr (MODE == SHIFTED) {
-        for (int k = 0; k < 2 * sh.ring && t < 32; ++k) {
-            T* buf = ring + k / 2 * slot_elems + k % 2 * sh.cap;
+        for (int k = 0; k < sh.ring && t < 32; ++k) {
+            T* buf = ring + k * slot_elems + sh.cap;
             const int e = t < 2 * U ? t - U : max(U, to - from - U) + t - 2 * U;
             if (e < sh.cap - U) buf[e] = 0;
         }
@@ -750,21 +773,28 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
             wv[j][i] = pair(a ? (w ? w[c] : T(1)) : T(0), b ? (w ? w[c + 1] : T(1)) : T(0));
             aw[j][i] = ab[j][i] = pair(T(0), T(0));
         }
+    // One warp asks for the whole units, another copies what is small: their instructions lie between two rows.
+    auto row_x = [&](int row) { return x + row * sh.pitch_x + from; };
+    auto row_g = [&](int row) { return dy + row * sh.pitch_g + from; };
+    auto small_of = [&](int row) { return small_copy<T, MODE>(row_x(row), row_g(row), to - from, sh.cap, 2 * sh.cap - U, mean + row, rstd + row, t & 31); };
+    const SmallCopy<T> small = small_of(slab);
+    const int64_t small_pitch = (t & 31) < 8 ? sh.pitch_x : (t & 31) < 16 ? sh.pitch_g : 1;
     auto fetch = [&](int row, int slot) {
-        if (t >= 32) return;
+        if (t >= 64) return;
         if (row < sh.spans) {
             T* base = ring + slot * slot_elems;
-            const T* px = x + row * sh.pitch_x + from;
-            const T* pg = dy + row * sh.pitch_g + from;
             if (t == 0) {
+                const T *px = row_x(row), *pg = row_g(row);
                 const Split<T> sx(px, to - from), sg(pg, to - from);
                 bar_expect(&full[slot], static_cast<uint32_t>((sx.mid + sg.mid) * sizeof(T)));
                 fetch_units(base, px, sx, &full[slot]);
                 fetch_units(base + sh.cap, pg, sg, &full[slot]);
-                copy_one(base + 2 * sh.cap - U, mean + row);
-                copy_one(base + 2 * sh.cap - U + 32, rstd + row);
+            } else if (t >= 32) {
+                SmallCopy<T> c = small;
+                if constexpr (MODE == MIXED) c = small_of(row);
+                else c.from += (row - slab) * small_pitch;
+                if (c.on) copy_one(base + c.to, c.from);
             }
-            if (MODE != ALIGNED && t < 16) fetch_ends(base + (t < 8 ? 0 : sh.cap), t < 8 ? px : pg, to - from, t & 7);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -776,7 +806,8 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
             mx = misalignment(x + row * sh.pitch_x + from);
             mg = misalignment(dy + row * sh.pitch_g + from);
         }
-        load_unit<T, MODE != MIXED>(col.some(j) ? base + mx : zeros, xh);
+        // behind the columns: the row's mean and no gradient (see ln_bwd_span_kernel)
+        load_unit<T, MODE != MIXED>(col.some(j) ? base + mx : ring + slot * slot_elems + 2 * sh.cap - U, xh);
         load_unit<T, MODE != MIXED>(col.some(j) ? base + sh.cap + mg : zeros, up);
         if (MODE == MIXED && !whole) {
             replace_outside(col.first(j), to, mu, xh);
@@ -799,13 +830,11 @@ __global__ void __launch_bounds__(SPAN_THREADS, 1) ln_bwd_wide_kernel(const T* _
             bar_wait(&full[slot], phase, limit, sh.gave_up);
             const T mu = ring[slot * slot_elems + 2 * sh.cap - U], rs = ring[slot * slot_elems + 2 * sh.cap - U + 32];
             const Pair<T> minus_mu = pair(-mu, -mu), rs2 = pair(rs, rs);
-            const bool far = far_from_zero(mu, rs);
             Pair<T> s0 = pair(T(0), T(0)), s1 = s0;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 Pair<T> xh[H], up[H];
                 load(row, slot, j, mu, minus_mu, rs2, xh, up);
-                if (MODE != MIXED && far) replace_outside(col.first(j), to, T(0), xh);
 #pragma unroll
                 for (int i = 0; i < H; ++i) {
                     const Pair<T> gv = up[i] * wv[j][i];
