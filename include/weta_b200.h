@@ -412,11 +412,13 @@ int64_t wb_adam_multi_offset(const WbAdamMulti* h, int index); /* offset_i; -1: 
  * tensor has none and is left as it is, its state too.  Only the pointers are kept. */
 int wb_adam_multi_set_grads(WbAdamMulti* h, const float* const* grads, int n);
 /* norm = sqrt(sum of all squares), summed in f64 in a fixed order; clip_scale (may be NULL) =
- * min(1, max_norm / (norm + 1e-6)).  Both are device scalars outside the parameters and the state. */
+ * min(1, max_norm / (norm + 1e-6)).  Both are device scalars outside the parameters and the state (in a gradient they would
+ * overwrite an element of it once the norm is taken). */
 int wb_adam_multi_grad_norm(WbAdamMulti* h, double max_norm, float* norm, float* clip_scale);
 /* Step t >= 1 (at t = 1 the old state is not read); lr and the rest may change from step to step.  The gradient is
  * multiplied by grad_scale (1: not at all) and, where device_grad_scale is not NULL, by that device scalar (not in a
- * parameter or the state), the two multiplied first.  With 32-bit state the results are wb_adam_step's, bit for bit. */
+ * parameter or the state), the two multiplied first.  With 32-bit state the results are wb_adam_step's, bit for bit.  A
+ * captured step keeps its t, its numbers and the gradients' addresses: replayed, it is that step again on what lies there. */
 int wb_adam_multi_step(WbAdamMulti* h, const WbAdamConfig* cfg, int64_t t, double grad_scale, const float* device_grad_scale);
 /* The moments as f32 [P] each (either may be NULL), in the state's order: what 8-bit state stands for. */
 int wb_adam_multi_read_state(WbAdamMulti* h, float* m, float* v);

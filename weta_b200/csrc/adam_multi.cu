@@ -250,9 +250,12 @@ struct AdamK8 {
 };
 
 // One warp takes a block of 256 elements, a lane the groups of four at 4 lane and 128 + 4 lane.
-// Bound by instruction issue (81 % of the slots): 101 M elements in 128 tensors took 562 us with conversions, roots and
-// quotients one at a time, 293 us now (251 us are their bytes).  One block per warp and five thread blocks per processor: with
-// two blocks in turn per warp 378 us, with four thread blocks 334 us, with six 322 us against 311 us at that stage.
+// Bound by instruction issue (82 % of the slots): 101 M elements in 128 tensors took 562 us with conversions, roots and
+// quotients one at a time, 286 us now (251 us are their bytes).  One block per warp and five thread blocks per processor: when
+// that took 311 us, four thread blocks took 334 us and six 322 us; two blocks in turn per warp took 378 us.
+// That holds where no moment is 0.  A lane that holds one, and every lane of a tensor's last block that is not full, takes
+// sqrtf and / for its eight elements and all roots of encode<false> again: the same tensors with nine rows of ten without
+// gradient since the first step 478 us, with every tenth gradient 0 579 us, with none at all 494 us.
 template <int N, bool FIRST>
 __global__ void __launch_bounds__(THREADS, 5) adam_multi8_kernel(const __grid_constant__ Table<N> tab, uint32_t* __restrict__ mc, uint32_t* __restrict__ vc,
                                                               float* __restrict__ ms, float* __restrict__ vs, const __grid_constant__ AdamK8 k8,

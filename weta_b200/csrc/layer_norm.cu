@@ -1352,7 +1352,7 @@ cudaError_t launch_spans(WbBackend* b, const SpanShape& sh, int groups, size_t s
     int64_t most = b->sm_count;
     if (CL > 1) {
         // Clusters that are resident at a time: not every processor group is a multiple of CL processors, and a cluster more than
-        // fit runs as a second wave ([4096, 16384] over clusters of 4: 461 us with 37 of them, 267 us with those that fit).
+        // fit runs as a second wave (backward, [2000, 30000] over clusters of 4: 254 us with 37 of them, 150 us with those that fit).
         int fit = 0;
         attr[n++] = cluster_attribute(CL);
         cfg.attrs = attr;
