@@ -119,3 +119,14 @@ def test_an_optimizer_of_a_closed_backend_refuses(fused):
         with pytest.raises(BackendError, match="backend is closed"):
             call()
     assert "step" not in inner.lib.calls and "read_state" not in inner.lib.calls
+
+
+def test_a_deferred_operand_given_to_the_wrapped_backend(fb):
+    """A deferred value has an address and a type like any storage, so the plain backend's call takes it as x and dy."""
+    rows, one, y = Layout.contiguous([1, N]), up(fb, np.zeros(1)), up(fb, np.zeros(N))
+    a = up(fb, np.arange(N))
+    layers.layer_norm_fwd(fb.inner, twice(fb, a), rows, DType.F32, 1, out=(y, None, None))
+    assert np.array_equal(down(fb, y), 2 * np.arange(N, dtype=F))
+    dx = up(fb, np.zeros(N))
+    layers.layer_norm_bwd(fb.inner, twice(fb, a), rows, twice(fb, y), rows, DType.F32, 1, None, one, one, out=(dx, None, None))
+    assert np.array_equal(down(fb, dx), 4 * np.arange(N, dtype=F))

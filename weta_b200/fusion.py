@@ -46,6 +46,7 @@ class LazyStorage:
     """What the caller holds in place of a device storage: the value exists at the latest when `.ptr` is read."""
 
     __slots__ = ("node", "backend", "__weakref__")
+    dtype = DType.F32  # no other calls are deferred
 
     def __init__(self, node: _Node, backend: "FusingBackend"):
         self.node, self.backend = node, backend
@@ -63,6 +64,12 @@ class LazyStorage:
     @property
     def length(self) -> int:
         return self.node.n
+
+    @property
+    def nbytes(self) -> int:
+        return 4 * self.node.n
+
+    _bytes = nbytes  # always known
 
 
 def _identity(layout: Layout, n: int) -> bool:
