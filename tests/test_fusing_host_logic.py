@@ -130,3 +130,65 @@ def test_a_deferred_operand_given_to_the_wrapped_backend(fb):
     dx = up(fb, np.zeros(N))
     layers.layer_norm_bwd(fb.inner, twice(fb, a), rows, twice(fb, y), rows, DType.F32, 1, None, one, one, out=(dx, None, None))
     assert np.array_equal(down(fb, dx), 4 * np.arange(N, dtype=F))
+
+
+def test_writing_to_a_value_leaves_the_storage_it_was_assigned_to(fb):
+    a, buf, nine = up(fb, np.arange(N)), up(fb, np.zeros(N)), up(fb, np.full(N, 9))
+    g = twice(fb, a)
+    fb.copy_strided(g, L, DType.F32, buf, L)
+    fb.copy_strided(nine, L, DType.F32, g, L)
+    assert np.array_equal(down(fb, g), np.full(N, 9, F)) and np.array_equal(down(fb, buf), 2 * np.arange(N, dtype=F))
+
+
+@pytest.mark.parametrize("dropped", [False, True])
+@pytest.mark.parametrize("how", ["copy", "layer norm", "step"])
+def test_what_still_reads_a_value_is_evaluated_before_its_storage_changes(fb, how, dropped):
+    """c = g + g waits while g is stored in a storage that is then written over."""
+    a, buf = up(fb, np.arange(N)), up(fb, np.zeros(N))
+    g = twice(fb, a)
+    c = twice(fb, g)
+    fb.copy_strided(g, L, DType.F32, buf, L)
+    if dropped:
+        del g
+    if how == "copy":
+        fb.copy_strided(up(fb, np.full(N, 9)), L, DType.F32, buf, L)
+    elif how == "layer norm":
+        layers.layer_norm_fwd(fb, up(fb, np.full(N, 9)), Layout.contiguous([1, N]), DType.F32, 1, out=(buf, None, None))
+    else:
+        opt = optim.AdamMulti(fb, [buf])
+        opt.set_grads([up(fb, np.full(N, 9))])
+        opt.step(1)
+    assert np.array_equal(down(fb, c), 4 * np.arange(N, dtype=F))
+    assert not np.array_equal(down(fb, buf), 2 * np.arange(N, dtype=F))
+
+
+def test_what_still_reads_a_stored_value_is_evaluated_before_it_is_written_over(fb):
+    g = twice(fb, up(fb, np.arange(N)))
+    c = twice(fb, g)
+    assert np.array_equal(down(fb, g), 2 * np.arange(N, dtype=F))
+    fb.copy_strided(up(fb, np.full(N, 9)), L, DType.F32, g, L)
+    assert np.array_equal(down(fb, c), 4 * np.arange(N, dtype=F)) and np.array_equal(down(fb, g), np.full(N, 9, F))
+
+
+def test_nothing_is_evaluated_for_readers_that_are_gone(fb):
+    a = up(fb, np.arange(N))
+    g = twice(fb, a)
+    c = twice(fb, twice(fb, g))  # the middle one is never stored
+    down(fb, g)
+    down(fb, c)
+    before = fb.programs
+    fb.copy_strided(a, L, DType.F32, g, L)
+    assert fb.programs == before
+
+
+def test_what_still_reads_a_gradient_that_got_its_own_storage(fb):
+    a, theta, buf = up(fb, np.arange(N)), up(fb, np.zeros(N)), up(fb, np.zeros(N))
+    g = twice(fb, a)
+    c = twice(fb, g)
+    fb.copy_strided(g, L, DType.F32, buf, L)
+    opt = optim.AdamMulti(fb, [theta])
+    opt.set_grads([g])
+    fb.copy_strided(up(fb, np.full(N, 9)), L, DType.F32, g, L)
+    opt.step(1)
+    assert np.array_equal(down(fb, c), 4 * np.arange(N, dtype=F)) and np.array_equal(down(fb, theta), np.full(N, -9, F))
+    assert np.array_equal(down(fb, buf), 2 * np.arange(N, dtype=F))

@@ -136,7 +136,7 @@ class FusingBackend:
                 st, node = s.concrete(), s.node
                 sharing = self._aliases.get(st.handle)
                 if sharing is not None and node in sharing:
-                    node.concrete = self._copy_out(st, Layout.contiguous([node.n]), node.n)
+                    self._part(node)
                     sharing.discard(node)
         return self.for_reading(*storages)
 
@@ -288,13 +288,26 @@ class FusingBackend:
         for nd, st in zip(outs_nodes, storages):
             nd.concrete = st if st is not None else into[0]
             nd.inputs = []  # the value exists: let go of the operands
+        for nd in outs_nodes:
+            self._note_readers(nd)
+
+    def _note_readers(self, node: _Node):
+        """What waits for a value that is stored now reads that storage."""
+        waiting = [c for c in node.consumers if c.concrete is None]
+        if waiting:
+            self._readers.setdefault(node.concrete.handle, weakref.WeakSet()).update(waiting)
+
+    def _part(self, node: _Node):
+        """Gives a value that shares a storage one of its own."""
+        node.concrete = self._copy_out(node.concrete, Layout.contiguous([node.n]), node.n)
+        self._note_readers(node)
 
     def _flush_readers(self, storage: DeviceStorage):
         """Called before `storage` is overwritten in place: evaluates every pending node that reads it, and gives every
         live handle whose value was written straight into it (see copy_strided) a storage of its own."""
         for node in list(self._aliases.pop(storage.handle, ())):
             if node.concrete is storage and node.handle_ref is not None and node.handle_ref() is not None:
-                node.concrete = self._copy_out(storage, Layout.contiguous([node.n]), node.n)
+                self._part(node)
         readers = self._readers.pop(storage.handle, None)
         if not readers:
             return
@@ -313,8 +326,8 @@ class FusingBackend:
         return self.inner.zeros(n, dt)
 
     def copy_strided(self, src, ls: Layout, dt, dst, ld: Layout):
-        dst_c = self._c(dst)
-        self._flush_readers(dst_c)
+        self._flush_readers(self._c(dst))
+        dst_c = self._c(dst)  # a value that shared another storage has one of its own now
         if (isinstance(src, LazyStorage) and src.node.concrete is None and dt == DType.F32 and _identity(ls, src.node.n) and _identity(ld, src.node.n)
                 and dst_c.length == src.node.n and not self._reads(src.node, dst_c)):
             # The pending expression is written straight into the destination (an in-place `assign` over a whole storage,
